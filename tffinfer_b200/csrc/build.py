@@ -44,8 +44,8 @@ def sources() -> List[str]:
     return sorted(f for f in os.listdir(CSRC_DIR) if f.endswith(".cu"))
 
 
-# Every model's: embedding, norms, products, sampling, state slots, the host side of TMA.
-CORE = ("elementwise", "gemm_f32", "gemm_simt", "gemm_tc", "gemm_tc_pair", "sampling", "tma_host")
+# Every model's: embedding, norms, products, control of logits, sampling, drafted trees, state slots, the host side of TMA.
+CORE = ("draft_tree", "elementwise", "gemm_f32", "gemm_simt", "gemm_tc", "gemm_tc_pair", "logit_control", "sampling", "tma_host")
 
 
 def chosen_sources(files: Optional[Iterable[str]]) -> List[str]:

@@ -70,7 +70,7 @@ class Engine:
         the step before read, so the host works while the device does.  Outputs therefore come one call
         late; ``has_unfinished`` stays true until the last ones have been handed out.  Whenever the host
         needs token values first -- a preempted request to recompute, pages about to run out, a
-        repetition penalty -- the step in flight is read before planning."""
+        penalty or a grammar -- the step in flight is read before planning."""
         outs: List[StepOutput] = self._held_outputs
         self._held_outputs = []
         sched = self.scheduler
@@ -100,11 +100,12 @@ class Engine:
                   "host": None, "event": None}
         samplers = record["samplers"]
         if samplers:
-            need_seen = any(r.params.repetition_penalty != 1.0 for r in samplers)
+            need_seen = any(r.params.needs_token_values for r in samplers)
             toks = self.sampler.sample(
                 logits, [r.params for r in samplers], [r.key for r in samplers],
                 [len(r.generated) for r in samplers],
-                [r.tokens for r in samplers] if need_seen else None)
+                [r.tokens for r in samplers] if need_seen else None,
+                [len(r.prompt) for r in samplers])
             record["tokens"] = toks
             if toks.is_cuda:
                 i = self._host_flip                    # two pinned buffers in turn: the one of the step
@@ -134,8 +135,8 @@ class Engine:
         return outs
 
     def _needs_token_values(self) -> bool:
-        return any(r.params.repetition_penalty != 1.0 for r in self.scheduler.running) or \
-            any(r.params.repetition_penalty != 1.0 for r in self.scheduler.waiting)
+        return any(r.params.needs_token_values for r in self.scheduler.running) or \
+            any(r.params.needs_token_values for r in self.scheduler.waiting)
 
     def _resolve(self, record) -> List[StepOutput]:
         drawn: Dict[Hashable, int] = {}

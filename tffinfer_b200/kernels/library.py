@@ -183,6 +183,15 @@ class CudaKernels:
                 raise KernelError("kernels take contiguous tensors")
 
     @staticmethod
+    def _need_here(*tensors) -> None:
+        """_need_cuda, and on the current device, whose stream the launch goes to."""
+        CudaKernels._need_cuda(*tensors)
+        here = torch._C._cuda_getDevice()
+        for t in tensors:
+            if t is not None and t.device.index != here:
+                raise KernelError(f"a tensor on cuda:{t.device.index} was given to a kernel on the current device, cuda:{here}")
+
+    @staticmethod
     def _cache_args(kv_cache, kv_layer: int):
         """(pointer, pages, layers, layer) of a paged cache [pages, layers, 2, kv heads, page, head] as the
         launchers take them.  The tensor is either contiguous as it reads (pages outermost), or that shape
@@ -815,6 +824,117 @@ class CudaKernels:
             return
         self._attention_generic_launch(q, batch, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window,
                                        softcap, sink, gates, keep)
+
+    TREE_MAX_NODES = 256          # of a request's tree of drafted tokens
+
+    def _tree_args(self, batch, parents, T: int) -> None:
+        """Checks what the kernels of drafted trees are given of a step."""
+        self._need_here(parents, batch.q_start, batch.pos_start)
+        B = batch.num_requests
+        if parents.dtype != torch.int32 or parents.numel() != T:
+            raise KernelError(f"parents are {T} int32 numbers, one a node")
+        if any(t.dtype != torch.int32 for t in (batch.q_start, batch.pos_start)) or batch.q_start.numel() < B + 1 or \
+                batch.pos_start.numel() < B:
+            raise KernelError("q_start and pos_start are int32, with an element a request (and one more)")
+        if batch.max_q_len > self.TREE_MAX_NODES:
+            raise KernelError(f"a request brings at most {self.TREE_MAX_NODES} nodes, got {batch.max_q_len}")
+
+    def attention_tree(self, q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale,
+                       window: int = 0, softcap: float = 0.0, sink=False, gates=None, keep: int = 0) -> None:
+        """Attention of a step whose requests bring trees of drafted tokens: q [T, nq*d] (normed, rotated) against the paged
+        cache, which holds the nodes' keys and values too -> out [T, nq*dv].  The other arguments as in ``attention_ext``.
+
+        Node i of a request (row batch.q_start[b] + i) lies in cache slot batch.pos_start[b] + i and sees the slots below
+        pos_start[b], its ancestors' and its own.  ``parents`` int32 [T]: an earlier node of the request, or -1 for a node that
+        follows the cached tokens.  A node whose chain of parents does not end at -1 (padding: -2) sees nothing, is seen by
+        none, and gives zeros.  A node's position, which counts for ``window`` and ``keep``, is pos_start[b] + its
+        ancestors (the queries and keys are rotated by it: ``batch.positions`` of such a step).  At most 256 nodes a request."""
+        self._need_here(q, block_table, out, gates)
+        T, B = q.shape[0], batch.num_requests
+        dc = kv_cache.shape[-1]
+        if not (kv_cache.dtype == q.dtype == out.dtype) or kv_cache.device != q.device:
+            raise KernelError("queries, cache and outputs have one type and lie on one device")
+        if tuple(q.shape) != (T, nq * d) or tuple(out.shape) != (T, nq * dv) or tuple(kv_cache.shape[2:]) != (2, nkv, page_size, dc) \
+                or dc < max(d, dv):
+            raise KernelError("queries are [T, nq * d], outputs [T, nq * dv], cache pages [2, nkv, page, at least d and dv]")
+        if gates is not None and (gates.dtype != torch.float32 or tuple(gates.shape) != (T, nq)):
+            raise KernelError("head gates are float32 [T, nq]")
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < B:
+            raise KernelError("the block table is int32 [requests, pages]")
+        if not 0 <= kv_layer < kv_cache.shape[1]:
+            raise KernelError(f"layer {kv_layer} of a cache of {kv_cache.shape[1]}")
+        self._tree_args(batch, parents, T)
+        if T == 0 or B == 0:
+            return
+        self._attention_tree_plain(q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window,
+                                   softcap, sink, gates, keep)
+
+    def _attention_tree_plain(self, q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window,
+                              softcap, sink, gates, keep, splits=None) -> None:
+        T, B = q.shape[0], batch.num_requests
+        c_ptr, _, c_layers, c_layer = self._cache_args(kv_cache, kv_layer)
+        sink_on, sink_val = self._sink_args(sink, nq)
+        if splits is None:
+            graph = getattr(batch, "graph_bucket", None) is not None
+            max_kv = block_table.shape[1] * page_size if graph else int(batch.max_kv_len)
+            splits = self.lib.tff_attention_tree_splits(_c_int(B), _c_int(batch.max_q_len), _c_int(max_kv), _c_int(nq), _c_int(nkv),
+                                                        _c_int(dv), _c_int(window), _c_int(keep), _c_int(self.NUM_SMS))
+        ws = torch.empty(T * nq * splits * (dv + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+        self._check(self.lib.tff_attention_tree(
+            _ptr(q), _c_int(_dt(q)), _ptr(batch.q_start), _ptr(batch.pos_start), _ptr(parents), _ptr(block_table),
+            _c_int(block_table.shape[1]), c_ptr, _c_int(c_layers), _c_int(c_layer), _c_int(page_size), _ptr(out), _c_int(T), _c_int(B),
+            _c_int(batch.max_q_len), _c_int(nq), _c_int(nkv), _c_int(d), _c_int(dv), _c_int(kv_cache.shape[-1]), _c_float(scale),
+            _c_int(window), _c_float(softcap), _c_int(1 if sink_on else 0), _ptr(sink_val), _ptr(gates), _c_int(keep), _c_int(splits),
+            _ptr(ws), self._stream()), "attention_tree")
+        self.launches += 2 if splits > 1 else 1
+
+    def accept_tree(self, batch, parents, drawn, path, emitted, count) -> None:
+        """Which drafted tokens a step's draws confirm.  ``drawn`` int32 [T]: the token drawn from the logits behind every node;
+        batch.token_ids: the nodes' own.  From node 0 of a request (the token drawn last, parent -1) on, the path goes to the first
+        child whose token is the one drawn behind the node, until there is none or W nodes are on it.
+        path int32 [B, W]: the path's nodes; emitted int32 [B, W]: the tokens drawn behind them, the request's new tokens;
+        both -1 beyond; count int32 [B]: their number (0 for a request without nodes)."""
+        tokens = batch.token_ids
+        T, B = tokens.numel(), batch.num_requests
+        self._need_here(tokens, drawn, path, emitted, count)
+        self._tree_args(batch, parents, T)
+        if any(t.dtype != torch.int32 for t in (tokens, drawn, path, emitted, count)):
+            raise KernelError("tokens, paths and counts are int32")
+        if drawn.numel() != T or path.dim() != 2 or path.shape[0] != B or path.shape != emitted.shape or count.numel() != B:
+            raise KernelError("a draw a node, and path and emitted [requests, width], count [requests]")
+        if B == 0 or path.shape[1] == 0:
+            count.zero_()
+            return
+        self._check(self.lib.tff_accept_tree(_ptr(tokens), _ptr(parents), _ptr(drawn), _ptr(batch.q_start), _c_int(T), _c_int(B),
+                                             _ptr(path), _ptr(emitted), _ptr(count), _c_int(path.shape[1]), self._stream()),
+                    "accept_tree")
+        self.launches += 1
+
+    def keep_path(self, kv_cache, batch, block_table, page_size, path, count) -> None:
+        """The keys and values of the accepted nodes go to where the next step expects them, in every layer of the cache
+        [pages, layers, planes, kv heads, page, head]: slot pos_start[b] + path[b, j] to slot pos_start[b] + j, j < count[b].
+        path and count as ``accept_tree`` gives them (a path's nodes ascend); the slots behind stay as they are."""
+        self._need_here(block_table, path, count, batch.pos_start)
+        B = batch.num_requests
+        if any(t.dtype != torch.int32 for t in (block_table, path, count, batch.pos_start)):
+            raise KernelError("block table, paths, counts and positions are int32")
+        if kv_cache.dim() != 6 or kv_cache.shape[4] != page_size:
+            raise KernelError("the cache is [pages, layers, planes, kv heads, page, head]")
+        if kv_cache.device != path.device:
+            raise KernelError("the cache is on another device")
+        if path.dim() != 2 or path.shape[0] != B or count.numel() != B or block_table.dim() != 2 or block_table.shape[0] < B or \
+                batch.pos_start.numel() < B:
+            raise KernelError("paths [requests, width], a count and a row of the block table a request")
+        if B == 0 or path.shape[1] <= 1 or kv_cache.numel() == 0:
+            return
+        self._cache_args(kv_cache, 0)                          # (refuses what is neither form of a cache)
+        pages, layers, planes, heads, _, d = kv_cache.shape
+        size = kv_cache.element_size()
+        self._check(self.lib.tff_keep_path(_ptr(kv_cache), _c_int(pages), _c_int(layers), _c_int(planes), _c_int(heads), _c_int(page_size),
+                                           _c_int(d * size), _c_int(kv_cache.stride(0) * size), _c_int(kv_cache.stride(1) * size),
+                                           _ptr(batch.pos_start), _ptr(block_table), _c_int(block_table.shape[1]), _ptr(path),
+                                           _ptr(count), _c_int(B), _c_int(path.shape[1]), self._stream()), "keep_path")
+        self.launches += 1
 
     def retain(self, h, w_in, freq, batch, state, decay, out, H, d, dv, k_scale: float, eps: float) -> None:
         """The whole of a retention mixer between its input rows and its output projection: one product for q, k, v
@@ -2243,4 +2363,29 @@ class CudaKernels:
         self._check(self.lib.tff_repetition_penalty(_ptr(logits), _ptr(rows), _ptr(tokens), _ptr(penalty),
                                                     _c_int(n), _c_int(logits.shape[1]), self._stream()),
                     "repetition_penalty")
+        self.launches += 1
+
+    def control_logits(self, logits, out, controls) -> None:
+        """out = logits (float32 [R, V]) under ``controls`` (sampling.LogitControls): penalties for repeated tokens, biases,
+        grammar masks.  ``out`` may be ``logits`` itself unless the rows are nodes of trees."""
+        c = controls
+        self._need_here(logits, out, c.row_start, c.settings, c.history, c.history_start, c.history_len, c.prompt_len, c.bias_start,
+                        c.bias_tokens, c.bias_values, c.mask, c.mask_row, c.parents, c.tokens)
+        R, V = logits.shape
+        if logits.dtype != torch.float32 or out.dtype != torch.float32 or out.shape != logits.shape:
+            raise KernelError("logits and outputs are float32 [rows, vocabulary]")
+        problem = c.problem(R, V)
+        if problem is not None:
+            raise KernelError(f"logit controls: {problem}")
+        apart = abs(out.data_ptr() - logits.data_ptr()) >= 4 * R * V
+        if not apart and (c.parents is not None or out.data_ptr() != logits.data_ptr()):
+            raise KernelError("the outputs of trees lie apart from the logits, others apart or in their place")
+        if R == 0 or V == 0:
+            return
+        self._check(self.lib.tff_control_logits(
+            _ptr(logits), _ptr(out), _c_int(R), _c_int(V), _c_int(c.row_start.numel() - 1), _ptr(c.row_start), _ptr(c.settings),
+            _ptr(c.history), _c_int(c.history.numel()), _ptr(c.history_start), _ptr(c.history_len), _ptr(c.prompt_len),
+            _ptr(c.bias_start), _ptr(c.bias_tokens), _ptr(c.bias_values), _c_int(c.bias_tokens.numel() if c.bias_tokens is not None else 0),
+            _ptr(c.mask), _c_int(c.mask.shape[0] if c.mask is not None else 0), _c_int(c.mask.shape[1] if c.mask is not None else 0),
+            _ptr(c.mask_row), _ptr(c.parents), _ptr(c.tokens), self._stream()), "control_logits")
         self.launches += 1

@@ -1,2 +1,3 @@
 from .params import SamplingParams, GREEDY, RANDOM, TOP_K, TOP_P
+from .controls import LogitControls
 from .sampler import Sampler, uniform_for

@@ -6,8 +6,11 @@ repetition penalty and multinomial draws exist unused (LLMSampler.cpp:21-54).  H
 they are honoured."""
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
-from typing import Tuple
+from typing import Callable, List, Optional, Tuple
+
+import numpy as np
 
 GREEDY = "greedy"
 RANDOM = "random"
@@ -27,6 +30,12 @@ class SamplingParams:
     seed: int = 0
     max_new_tokens: int = 16
     eos_token_ids: Tuple[int, ...] = ()
+    frequency_penalty: float = 0.0     # taken off a token's logit for every time it was generated
+    presence_penalty: float = 0.0      # taken off a token's logit once it was generated
+    logit_bias: Tuple[Tuple[int, float], ...] = ()        # (token, what is added to its logit; -infinity bans it)
+    # a grammar: the generated tokens so far -> 32-bit words with a bit for every allowed token (token t: bit t % 32 of word
+    # t // 32), or None for no limit
+    token_mask: Optional[Callable[[List[int]], Optional[np.ndarray]]] = None
 
     def __post_init__(self):
         if self.type not in STRATEGIES:
@@ -37,8 +46,24 @@ class SamplingParams:
             raise ValueError("top_k >= 0, 0 < top_p <= 1 and 0 <= min_p < 1 are required")
         if self.repetition_penalty <= 0:
             raise ValueError("repetition_penalty must be > 0")
+        if not (math.isfinite(self.frequency_penalty) and math.isfinite(self.presence_penalty)):
+            raise ValueError("frequency_penalty and presence_penalty must be finite")
+        if any(t < 0 or not v < math.inf for t, v in self.logit_bias):
+            raise ValueError("logit_bias is pairs of a token id and a finite number or -infinity")
         if self.max_new_tokens < 0:
             raise ValueError("max_new_tokens must be >= 0")
+
+    @property
+    def controls_logits(self) -> bool:
+        """Whether the logits are changed by more than a repetition penalty ahead of the draw."""
+        return (self.frequency_penalty != 0.0 or self.presence_penalty != 0.0 or len(self.logit_bias) > 0
+                or self.token_mask is not None)
+
+    @property
+    def needs_token_values(self) -> bool:
+        """Whether a draw depends on which tokens the request has had."""
+        return (self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0 or self.presence_penalty != 0.0
+                or self.token_mask is not None)
 
     @property
     def is_greedy(self) -> bool:

@@ -12,6 +12,7 @@ from typing import Optional, Sequence
 import numpy as np
 import torch
 
+from .controls import LogitControls
 from .params import SamplingParams
 
 _M64 = (1 << 64) - 1
@@ -39,15 +40,21 @@ class Sampler:
         self.device = device
 
     def sample(self, logits: torch.Tensor, params: Sequence[SamplingParams], request_keys: Sequence[int],
-               indices: Sequence[int], seen_tokens: Optional[Sequence[Sequence[int]]] = None) -> torch.Tensor:
+               indices: Sequence[int], seen_tokens: Optional[Sequence[Sequence[int]]] = None,
+               prompt_lens: Optional[Sequence[int]] = None) -> torch.Tensor:
         """logits float32 [R, V]; row r belongs to a request with params[r], key request_keys[r],
         generating its token number indices[r]; seen_tokens[r] (prompt + generated) is needed only
-        when a repetition penalty is set.  Returns int32 [R] on the device."""
+        when a penalty or a grammar is set (params[r].needs_token_values), prompt_lens[r] (how many of
+        them are the prompt) only for another one than the repetition penalty.  Returns int32 [R] on the device."""
         R = logits.shape[0]
         out = torch.empty(R, dtype=torch.int32, device=logits.device)
         if R == 0:
             return out
-        if any(p.repetition_penalty != 1.0 for p in params):
+        if any(p.controls_logits for p in params):
+            seen = [list(t) if p.needs_token_values else [] for p, t in zip(params, seen_tokens or [[]] * R)]
+            lens = [n if p.needs_token_values else 0 for p, n in zip(params, prompt_lens or [0] * R)]
+            self.ops.control_logits(logits, logits, LogitControls.of(params, lens, seen, logits.shape[1], logits.device))
+        elif any(p.repetition_penalty != 1.0 for p in params):
             self._penalize(logits, params, seen_tokens)
         if all(p.is_greedy for p in params):
             self.ops.argmax(logits, out)
