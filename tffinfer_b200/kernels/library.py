@@ -866,6 +866,20 @@ class CudaKernels:
         self._tree_args(batch, parents, T)
         if T == 0 or B == 0:
             return
+        if q.dtype == torch.bfloat16 and d == dv == dc and d in (64, 128):
+            c_ptr, c_pages, c_layers, c_layer = self._cache_args(kv_cache, kv_layer)
+            sink_on, sink_val = self._sink_args(sink, nq)
+            ws = torch.empty(self.lib.tff_attention_tree_tc_workspace(_c_int(batch.max_q_len), _c_int(nq), _c_int(nkv), _c_int(d)),
+                             dtype=torch.uint8, device=q.device)
+            status = self.lib.tff_attention_tree_tc(
+                _ptr(q), _ptr(batch.q_start), _ptr(batch.pos_start), _ptr(parents), _ptr(block_table), _c_int(block_table.shape[1]),
+                c_ptr, _c_int(c_pages), _c_int(c_layers), _c_int(c_layer), _c_int(page_size), _ptr(out), _c_int(T), _c_int(B),
+                _c_int(batch.max_q_len), _c_int(nq), _c_int(nkv), _c_int(d), _c_float(scale), _c_int(window), _c_float(softcap),
+                _c_int(1 if sink_on else 0), _ptr(sink_val), _ptr(gates), _c_int(keep), _ptr(ws), self._stream())
+            if status != -2:                              # (what the kernel does not take, the general one does)
+                self._check(status, "attention_tree_tc")
+                self.launches += 2
+                return
         self._attention_tree_plain(q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window,
                                    softcap, sink, gates, keep)
 
