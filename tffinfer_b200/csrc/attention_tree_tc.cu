@@ -43,13 +43,14 @@ using tc5::tc_fence_after;
 using tc5::tmem_ld16;
 using tc5::tmem_ld_wait;
 
-constexpr int BLOCK_M = 128, BLOCK_N = 64, BARS_PER_TILE = 16, JOIN_ROWS = 16;
+constexpr int BLOCK_M = 128, BLOCK_N = 64, BARS_PER_TILE = 16, JOIN_ROWS = 32;
 constexpr float RESCALE_THRESHOLD = 8.0f;            // in log2 units
 
 struct TreeTcParams {
     const bf16* q; bf16* out;
     const int *q_start, *pos_start, *parents, *block_table;
-    int requests, table_width, cache_layers, layer, page_shift, nq, nkv, window, keep, least;
+    int requests, table_width, cache_layers, layer, page_shift, nq, nkv, window, keep, least, extra, whole;
+    int group; unsigned group_inverse;               // query heads a kv head, and what a row number is multiplied by for its node
     float scale_log2, scale_over_cap, cap_log2;
     int sink; const float *sink_val, *gate;
     float *part_o, *part_ml; int4* joins;
@@ -71,96 +72,131 @@ struct TreeCfg {
     static constexpr int kExchange = QT * 2 * BLOCK_M * 4;          // a float of every row from either group
     static constexpr int kParents = TREE_MAX_NODES * 2;
     static constexpr int kBars = 2 * kStages + BARS_PER_TILE * QT;
-    static constexpr int kSmem = QT * kQBytes + kStages * kStageBytes + kExchange + kParents + 8 * kBars + 16;
+    static constexpr int kSmem = QT * kQBytes + kStages * kStageBytes + kExchange + kParents + 8 * kBars + 8 + 2 * 80;
     static constexpr int kThreads = (8 * QT + 1 + QT) * 32;
     static_assert(kSmem <= 227 * 1024, "shared memory of the tree attention kernel");
 };
 
-// A request's walk.
+// A request's walk: the blocks of 64 keys that its rows see, for each of its tiles.
 struct Walk {
-    int q0, nodes, ctx, lo, tiles, count;
-    template <typename P>
-    __device__ __forceinline__ Walk(const P& p, int b, int tile_rows) {
+    int q0 = 0, nodes = 0, ctx = 0, lo = 0, tiles = 0, count = 0;
+    __device__ __forceinline__ void read(const TreeTcParams& p, int b, int tile_rows) {
         q0 = p.q_start[b];
         nodes = max(0, min(p.q_start[b + 1] - q0, TREE_MAX_NODES));
         ctx = p.pos_start[b];
         lo = p.window > 0 ? max(0, ctx - p.window + 1) : 0;         // the first position that a root sees
-        tiles = (nodes * (p.nq / p.nkv) + tile_rows - 1) / tile_rows;
+        tiles = (nodes * p.group + tile_rows - 1) / tile_rows;
         count = tiles > 0 ? keys(p.keep).count : 0;
     }
     __device__ __forceinline__ int hi() const { return ctx + nodes - 1; }
     __device__ __forceinline__ KeyWalk keys(int keep) const { return KeyWalk(keep, BLOCK_N, lo / BLOCK_N, hi() / BLOCK_N); }
-    __device__ __forceinline__ long long blocks() const { return (long long)tiles * count; }
 };
 
-// A CTA's share of the line of blocks, piece by piece.  Every warp goes through it by itself, with all its lanes.
-template <int ROWS>
+// How a line of ``all`` units is shared out: the first ``rest`` CTAs have one unit more than the others.
+struct Shares {
+    int ctas, each, rest;
+    __device__ __forceinline__ Shares(int all, int least) {
+        ctas = min((int)gridDim.x, max(1, all / least));
+        each = all / ctas;
+        rest = all - each * ctas;
+    }
+    __device__ __forceinline__ int begin(int cta) const { return cta >= ctas ? each * ctas + rest : cta * each + min(cta, rest); }
+    __device__ __forceinline__ int owner(int unit) const {
+        const int more = rest * (each + 1);
+        return unit < more ? unit / (each + 1) : rest + (unit - more) / each;
+    }
+};
+
+// A CTA's share, piece by piece.  A walk has ``extra`` units ahead of its blocks, for what a piece costs beside them: a CTA of
+// several pieces has fewer blocks.  ``whole``: a share is the walks that begin in it.
 struct Pieces {
-    const TreeTcParams& p;
-    long long first, left, line;                     // the share's first block, blocks behind the present piece, blocks a kv head
-    int ctas;                                        // that have a share
-    int b, kvh, tile, at, nb;                        // the piece: request, kv head, tile; its first block of the walk, its blocks
+    int left = 0;                                    // units of the share behind the present piece
+    int b = 0, kvh = 0, tile = 0, at = 0, nb = 0;    // the piece: request, kv head, tile; its first block of the walk, its blocks
+    int unit = 0;                                    // of the walk, behind the present piece
     Walk w;
-    __device__ __forceinline__ Pieces(const TreeTcParams& p_) : p(p_), b(0), kvh(0), tile(0), at(0), nb(0), w(p_, 0, ROWS) {
+    // A warp's, with all its lanes; returns the line's units and the share's first one.
+    template <int ROWS>
+    __device__ __forceinline__ int2 start(const TreeTcParams& p) {
         const int lane = threadIdx.x & 31;
-        auto sum_of = [&](int r0) -> long long {     // inclusive sums of 32 requests' blocks
-            long long s = r0 + lane < p.requests ? Walk(p, r0 + lane, ROWS).blocks() : 0;
+        Walk v;
+        auto sum_of = [&](int r0) -> int {           // inclusive sums of 32 requests' units
+            v = Walk();
+            if (r0 + lane < p.requests) v.read(p, r0 + lane, ROWS);
+            int s = v.count > 0 ? v.tiles * (v.count + p.extra) : 0;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
-                const long long before = __shfl_up_sync(0xffffffffu, s, o);
+                const int before = __shfl_up_sync(0xffffffffu, s, o);
                 if (lane >= o) s += before;
             }
             return s;
         };
-        const long long head = sum_of(0);
-        line = __shfl_sync(0xffffffffu, head, 31);
+        const int head = sum_of(0);
+        int line = __shfl_sync(0xffffffffu, head, 31);                 // units a kv head
         for (int r0 = 32; r0 < p.requests; r0 += 32) line += __shfl_sync(0xffffffffu, sum_of(r0), 31);
-        const long long all = line * p.nkv;
-        ctas = (int)min((long long)gridDim.x, max(1ll, all / p.least));
-        first = share(blockIdx.x);
-        left = (int)blockIdx.x < ctas ? share(blockIdx.x + 1) - first : 0;
-        if (left <= 0) { left = 0; return; }
-        kvh = (int)(first / line);
-        long long rest = first % line;
+        const Shares sh(line * p.nkv, p.least);
+        const int first = sh.begin(blockIdx.x);
+        left = sh.begin(blockIdx.x + 1) - first;
+        if (left <= 0) { left = 0; return make_int2(line * p.nkv, first); }
+        kvh = first / line;
+        int rest = first - kvh * line;
         for (int r0 = 0; r0 < p.requests; r0 += 32) {
-            const long long s = r0 == 0 ? head : sum_of(r0);
+            const int s = r0 == 0 && p.requests <= 32 ? head : sum_of(r0);
             const unsigned behind = __ballot_sync(0xffffffffu, rest < s);
             if (behind) {
                 const int src = __ffs(behind) - 1;
                 b = r0 + src;
-                const long long before = __shfl_sync(0xffffffffu, s, max(src - 1, 0));
+                const int before = __shfl_sync(0xffffffffu, s, max(src - 1, 0));
                 rest -= src > 0 ? before : 0;
+                w.q0 = __shfl_sync(0xffffffffu, v.q0, src); w.nodes = __shfl_sync(0xffffffffu, v.nodes, src);
+                w.ctx = __shfl_sync(0xffffffffu, v.ctx, src); w.lo = __shfl_sync(0xffffffffu, v.lo, src);
+                w.tiles = __shfl_sync(0xffffffffu, v.tiles, src); w.count = __shfl_sync(0xffffffffu, v.count, src);
                 break;
             }
             rest -= __shfl_sync(0xffffffffu, s, 31);
         }
-        w = Walk(p, b, ROWS);
-        tile = (int)(rest / w.count);
-        at = (int)(rest % w.count);
+        const int span = w.count + p.extra;
+        tile = rest / span;
+        unit = rest - tile * span;
+        if (p.whole && unit > 0) {                   // (that walk is another CTA's)
+            left -= span - unit;
+            unit = span;
+        }
+        at = max(0, unit - p.extra);
+        return make_int2(line * p.nkv, first);
     }
-    __device__ __forceinline__ long long share(int cta) const { return line * p.nkv * cta / ctas; }
     // The next piece; false behind the last.
-    __device__ __forceinline__ bool next() {
-        at += nb;
-        if (nb > 0 && at == w.count) {
-            at = 0;
+    template <int ROWS>
+    __device__ __forceinline__ bool next(const TreeTcParams& p) {
+        if (left <= 0) return false;
+        if (unit == w.count + p.extra) {
+            unit = 0;
             if (++tile == w.tiles) {
                 tile = 0;
-                if (left > 0) {
-                    do {
-                        if (++b == p.requests) { b = 0; ++kvh; }
-                        w = Walk(p, b, ROWS);
-                    } while (w.count == 0);
-                }
+                do {
+                    if (++b == p.requests) { b = 0; ++kvh; }
+                    w.read(p, b, ROWS);
+                } while (w.count == 0);
             }
         }
-        if (left <= 0) return false;
-        nb = (int)min(left, (long long)(w.count - at));
-        left -= nb;
-        return true;
+        const int end = p.whole ? w.count + p.extra : min(unit + left, w.count + p.extra);
+        at = max(0, unit - p.extra);
+        nb = max(0, end - p.extra) - at;
+        left -= end - unit;
+        unit = end;
+        return nb > 0;                               // (none: the share ends ahead of the walk's first block)
     }
-    __device__ __forceinline__ bool whole() const { return at == 0 && nb == w.count; }
+    __device__ __forceinline__ bool all() const { return at == 0 && nb == w.count; }
 };
+
+// A piece that the softmax warps are at, in shared memory: they have no registers for it.
+struct Present {
+    Pieces p;
+    KeyWalk keys;
+    int go, stage, fresh;                            // whether there is a piece; the stage of its first block; whether its request is another than before
+};
+
+// A row's node.
+__device__ __forceinline__ int node_of(const TreeTcParams& p, int row) { return p.group == 1 ? row : (int)__umulhi((unsigned)row, p.group_inverse); }
 
 // below(k): the first k of 64 bits.
 __device__ __forceinline__ uint64_t below(int k) { return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1; }
@@ -196,8 +232,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
     auto ref_bar = [&](int x, int g, int q) { return tile_bar(x, 8 + 4 * g + q); };
     volatile uint32_t* tmem_slot = (volatile uint32_t*)(smem + BARS_AT + 8 * Cfg::kBars);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    Present* present = (Present*)(tmem_slot + 2);                // [2]: the piece, and the next one
+    static_assert(sizeof(Present) <= 80, "a piece's place");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int G = p.nq / p.nkv;
+    const int G = p.group;
 
     if (tid == 0) {
         for (int s = 0; s < NSTAGES; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), QT); }
@@ -219,28 +257,23 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
     constexpr uint32_t tmem_base = 0;
     pdl_launch_dependents();
     pdl_wait();
-    Pieces<ROWS> piece(p);
+    Pieces piece;
+    const int2 line = piece.template start<ROWS>(p);
 
     if (warp == LOAD_WARP) {
         // ------------------------------------------------------------ TMA producer
-        if (lane == 0) {
-            // the walk that this share's first piece ends, if others began it: joined by the second kernel
-            int4 join = make_int4(-1, 0, 0, 0);
-            if (piece.left > 0 && piece.at > 0 && piece.w.count - piece.at <= piece.left) {
-                const long long start = piece.first - piece.at;
-                int c = (int)(start * piece.ctas / (piece.line * p.nkv));
-                while (c > 0 && piece.share(c) > start) --c;
-                while (piece.share(c + 1) <= start) ++c;
-                join = make_int4(piece.b, piece.kvh, piece.tile, c);
-            }
-            p.joins[blockIdx.x] = join;
+        // the walk that this share's first piece ends, if others began it: joined by the second kernel
+        int4 join = make_int4(-1, 0, 0, 0);
+        int begun = -1;
+        if (piece.left > 0 && piece.at > 0 && piece.w.count - piece.at <= piece.left) {
+            join = make_int4(piece.b, piece.kvh, piece.tile, 0);
+            begun = line.y - piece.unit + p.extra;           // (the unit of the walk's first block)
         }
-        __syncwarp();
         const int ppb = BLOCK_N >> p.page_shift;
         int s = 0;
         uint32_t round = 0;
         bool ok = true;
-        while (ok && piece.next()) {
+        while (ok && piece.template next<ROWS>(p)) {
             const KeyWalk walk = piece.w.keys(p.keep);
             const int* table = p.block_table + (size_t)piece.b * p.table_width;
             const int table_end = piece.w.hi() >> p.page_shift;
@@ -252,6 +285,8 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
             };
             for (int i = 0; i < piece.nb; ++i) {
                 if (round > 0 && !(ok = mbar_wait_warp(kv_empty(s), (round - 1) & 1, abort_flag))) break;
+                // the first queries are on their way before more than two blocks are asked for: every CTA begins with both
+                if (round == 0 && i == 2 && s == 2 && !(ok = mbar_wait_warp(q_ready(0), 0, abort_flag))) break;
                 const int first = walk.block(piece.at + i) * BLOCK_N >> p.page_shift;       // (a block's pages lie in one run of 32)
                 if (first >> 5 != chunk) {
                     held = first >> 5 == chunk + 1 && chunk >= 0 ? ahead : entry(first >> 5);
@@ -270,6 +305,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                 if (++s == NSTAGES) { s = 0; ++round; }
             }
         }
+        if (!p.whole && lane == 0) {
+            if (begun >= 0) join.w = Shares(line.x, p.least).owner(begun);
+            p.joins[blockIdx.x] = join;
+        }
     } else if (warp >= ISSUE_WARP) {
         // -------------------------------------------------------------- MMA issuers, one per tile
         auto issue = [&](auto which) {
@@ -284,7 +323,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
             uint32_t phase = 0, phase_q = 0, phase_s = 1;          // of the ring, the queries, s_free (nothing to wait for at first)
             uint32_t phase_p[2] = {0, 0};
             int st = 0, st_pv = 0;                                 // stages of S(n) and of PV(n - 2)
-            while (ok && piece.next()) {
+            while (ok && piece.template next<ROWS>(p)) {
                 if (piece.tile * ROWS + x * BLOCK_M >= piece.w.nodes * G) {
                     // a tile without rows gives the stages back as they arrive
                     for (int n = 0; n < piece.nb && ok; ++n) {
@@ -335,7 +374,6 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
         const int x = warp >> 3, g = (warp >> 2) & 1;              // query tile and group of this warp: it has a piece's blocks g, g + 2, ...
         const int q = warp & 3;                                    // TMEM lane quarter this warp may touch
         const int r = q * 32 + lane;                               // row of the tile = TMEM lane
-        const int tt = tid & 127;                                  // within the group
         const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + x * 256;
         const uint32_t t_s = t_row, t_p = t_row + 64 + g * 32, t_o = t_row + 128;
         // the two warps that have a row between them; all that read the parents and the queries' place
@@ -346,76 +384,90 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
         const float scale_log2 = p.cap_log2 > 0.f ? p.cap_log2 : p.scale_log2;
         // completions so far, mod 2: of the barriers of the own group, and of the other's
         uint32_t n_own = 0, n_other = 0;
-        int stage = 0;                                             // of the piece's first block
-        int parents_of = -1;
         bool ok = true;
-        while (piece.next()) {
-            const int q0 = piece.w.q0, ctx = piece.w.ctx, nodes = piece.w.nodes, hi = piece.w.hi(), nb = piece.nb;
-            const KeyWalk walk = piece.w.keys(p.keep);
-            const int R0 = piece.tile * ROWS + x * BLOCK_M, R = R0 + r, rows_total = nodes * G;
-            const bool tile_active = R0 < rows_total;
-            const int tok = R / G, head = piece.kvh * G + R % G;
-            const int rows_left = min(32, rows_total - (R - lane));            // rows of this warp's 32 that exist
+        if (tid == 0) {
+            present->go = piece.template next<ROWS>(p);
+            present->p = piece;
+            present->keys = piece.w.keys(p.keep);
+            present->stage = 0;
+            present->fresh = 1;
+        }
+        soft_sync();
+        for (const Present* now = present;; now = present + (now == present)) {
+            if (!now->go) break;
+            const int rows_total = now->p.w.nodes * G;
+            auto row_of = [&]() { return now->p.tile * ROWS + x * BLOCK_M + r; };
+            auto left_of = [&]() { return min(32, now->p.w.nodes * G - (row_of() - lane)); };      // rows of this warp's 32 that exist
+            const int R = row_of(), rows_left = left_of(), tok = node_of(p, R);
+            const bool tile_active = R - r < rows_total;
             // ---------------------------------- queries and parents; half of the columns of this warp's rows a group
             constexpr int RC = D / 16;                             // 16-byte chunks of a row that a group has
             uint4 u[RC];
-            if (tile_active) {
+            if (rows_left > 0) {
+                // (rows that do not exist take the last one's place: no load waits for another)
+                const bf16* from = p.q + ((size_t)now->p.w.q0 * p.nq + now->p.kvh * G) * D + g * RC * 8;
 #pragma unroll
                 for (int i = 0; i < RC; ++i) {
-                    const int row = (i * 32 + lane) / RC, c = g * RC + (i * 32 + lane) % RC;
-                    const int t = __shfl_sync(0xffffffffu, tok, row), h = __shfl_sync(0xffffffffu, head, row);
-                    u[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (row < rows_left)
-                        u[i] = __ldcg(reinterpret_cast<const uint4*>(p.q + ((size_t)(q0 + t) * p.nq + h) * D + c * 8));
+                    const int row = min((i * 32 + lane) / RC, rows_left - 1), c = (i * 32 + lane) % RC;
+                    const int of = R - lane + row, t = node_of(p, of);
+                    u[i] = __ldcg(reinterpret_cast<const uint4*>(from + ((size_t)t * p.nq + (of - t * G)) * D + c * 8));
                 }
             }
-            if (parents_of != piece.b) {
-                // (every softmax thread goes through the same pieces)
-                for (int i = tid; i < nodes; i += SOFT) parent[i] = tree_parent(__ldcg(p.parents + q0 + i), i);
+            if (now->fresh) {
+                const int nodes = now->p.w.nodes;
+                for (int i = tid; i < nodes; i += SOFT) parent[i] = tree_parent(__ldcg(p.parents + now->p.w.q0 + i), i);
                 soft_sync();
-                const bool gone = tid < nodes && tree_depth(parent, tid) < 0;
-                static_assert(SOFT >= TREE_MAX_NODES, "a thread a node");
-                soft_sync();
-                if (gone) parent[tid] = -2;                        // whoever follows it is marked as well
-                soft_sync();
-                parents_of = piece.b;
             }
-            const int depth = tile_active && R < rows_total ? tree_depth(parent, tok) : -1;
-            const bool rv = depth >= 0;                            // a row of a node that is there
-            const int pr = ctx + depth;
-            const int lo_r = p.window > 0 ? max(0, pr - p.window + 1) : 0;
+            const int depth = R < rows_total ? tree_depth(parent, tok) : -1;   // (-1: a row of no node that is there)
             if (tile_active) {
                 uint8_t* dst = smem + x * Cfg::kQBytes + q * 32 * 128;
 #pragma unroll
                 for (int i = 0; i < RC; ++i) {
                     const int row = (i * 32 + lane) / RC, c = g * RC + (i * 32 + lane) % RC;
                     // padding has queries of zeros: whatever it brought, its scores are finite
-                    if (!__shfl_sync(0xffffffffu, (int)rv, row)) u[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (__shfl_sync(0xffffffffu, depth, row) < 0) u[i] = make_uint4(0u, 0u, 0u, 0u);
                     *reinterpret_cast<uint4*>(dst + (c >> 3) * (BLOCK_M * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = u[i];
                 }
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_ready(x));
             }
+            if (warp == 0) {                                       // the next piece, while the first products run
+                Pieces next = now->p;
+                const bool go = next.template next<ROWS>(p);
+                Present* to = present + (now == present);
+                if (lane == 0) {
+                    to->fresh = next.b != now->p.b;
+                    to->stage = (now->stage + now->p.nb) % NSTAGES;
+                    to->go = go;
+                    to->p = next;
+                    to->keys = next.w.keys(p.keep);
+                }
+                __syncwarp();
+            }
             float m_used = -INFINITY, l = 0.f;
-            const int nb_x = tile_active ? nb : 0;
+            const int nb_x = tile_active ? now->p.nb : 0;
             for (int j = g; j < nb_x && ok; j += 2) {
                 ok = mbar_wait_warp(s_full(x, g), n_own, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                const int n_first = walk.block(piece.at + j) * BLOCK_N;
+                const int n_first = now->keys.block(now->p.at + j) * BLOCK_N;
                 // Masked or capped scores are written back over the raw ones, so that the pass below is the same for every block.
                 // Rows that are not there are not stored: they need no mask.
-                const bool some_nodes = n_first + BLOCK_N > ctx;
-                const bool masked = some_nodes || !__all_sync(0xffffffffu, !rv || n_first >= lo_r || n_first + BLOCK_N <= p.keep);
+                const bool some_nodes = n_first + BLOCK_N > now->p.w.ctx;
+                bool masked = some_nodes;
+                if (p.window > 0 && !some_nodes)
+                    masked = !__all_sync(0xffffffffu, depth < 0 || n_first > now->p.w.ctx + depth - p.window || n_first + BLOCK_N <= p.keep);
                 if (masked || p.cap_log2 > 0.f) {
                     uint64_t seen = ~0ull;
-                    if (masked && rv) {
-                        seen = below(ctx - n_first) & (~below(lo_r - n_first) | below(p.keep - n_first));
+                    if (masked && depth >= 0) {
+                        const int ctx = now->p.w.ctx;
+                        int pos = ctx + depth;
+                        const int lo = p.window > 0 ? pos - p.window + 1 : 0;
+                        seen = below(ctx - n_first) & (~below(lo - n_first) | below(p.keep - n_first));
                         if (some_nodes) {
-                            int pos = pr;
                             for (int a = tok; a >= 0 && ctx + a >= n_first; a = parent[a], --pos)
-                                if (ctx + a < n_first + BLOCK_N && (pos >= lo_r || pos < p.keep)) seen |= 1ull << (ctx + a - n_first);
+                                if (ctx + a < n_first + BLOCK_N && (pos >= lo || pos < p.keep)) seen |= 1ull << (ctx + a - n_first);
                         }
                     }
                     const uint32_t seen_lo = (uint32_t)seen, seen_hi = (uint32_t)(seen >> 32);
@@ -465,15 +517,19 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                     if (!ok) break;
                     tc_fence_after();
                 }
-                if (some_nodes || walk.ragged(piece.at + j)) {
+                if (some_nodes || now->keys.ragged(now->p.at + j)) {
                     // value rows that no row may see (behind the last node, between the kept ones and the first window, of
                     // padding) are cleared, since slots and unfetched shared memory may hold anything; the warps of both tiles
                     // do it (the same zeros), so that each tile's products wait for its own warps only
-                    uint8_t* rows = gKV + ((stage + j) % NSTAGES) * STAGE_BYTES + V_AT;
-                    for (int idx = tt; idx < BLOCK_N * CH; idx += 128) {
-                        const int kr = idx / CH, c = idx % CH;
-                        const int n = n_first + kr;
-                        if (n > hi || (n < piece.w.lo && n >= p.keep) || (n >= ctx && parent[n - ctx] == -2))
+                    uint8_t* rows = gKV + ((now->stage + j) % NSTAGES) * STAGE_BYTES + V_AT;
+                    const int ctx = now->p.w.ctx, hi = now->p.w.hi(), lo = now->p.w.lo;
+                    auto unseen = [&](int n) { return n > hi || (n < lo && n >= p.keep) || (n >= ctx && tree_depth(parent, n - ctx) < 0); };
+                    const unsigned first = __ballot_sync(0xffffffffu, unseen(n_first + lane)), second = __ballot_sync(0xffffffffu, unseen(n_first + 32 + lane));
+                    // a quarter of the rows a warp of the group, two rows at a time
+#pragma unroll 1
+                    for (int i = 0; i < BLOCK_N / 4; i += 32 / CH) {
+                        const int kr = q * (BLOCK_N / 4) + i + lane / CH, c = lane % CH;
+                        if ((kr < 32 ? first >> kr : second >> (kr - 32)) & 1u)
                             *reinterpret_cast<uint4*>(rows + (c >> 3) * 1024 + (kr >> 3) * GROUP + (kr & 7) * 128 + (((c & 7) ^ (kr & 7)) << 4)) =
                                 make_uint4(0u, 0u, 0u, 0u);
                     }
@@ -553,11 +609,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                 tc_fence_after();
                 // through shared memory, where the queries lay (every S is finished), 32 rows a warp
                 uint8_t* rows = smem + x * Cfg::kQBytes + (g * 4 + q) * (32 * D);
-                if (piece.whole()) {
+                if (now->p.all()) {
+                    const int rows_left = left_of(), t = now->p.w.q0 + tok, head = now->p.kvh * G + (row_of() - tok * G);
                     if (p.sink && l > 0.f) l += exp2f(attn_sink_log2(p.sink_val, head) - m_used);       // a key without a value
-                    const bool some = rv && l > 0.f;               // (a padding row's sums may be anything)
+                    const bool some = depth >= 0 && l > 0.f;               // (a padding row's sums may be anything)
                     float inv = some ? 1.f / l : 0.f;
-                    if (p.gate && some) inv *= __ldcg(p.gate + (size_t)(q0 + tok) * p.nq + head);
+                    if (p.gate && some) inv *= __ldcg(p.gate + (size_t)t * p.nq + head);
                     auto cell = [&](int row, int c) { return rows + row * D + ((c ^ (RC == 8 ? row & 7 : (row >> 1) & 3)) << 4); };
 #pragma unroll
                     for (int half = 0; half < RC / 4; ++half) {
@@ -580,42 +637,36 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
 #pragma unroll
                     for (int i = 0; i < RC; ++i) {
                         const int row = (i * 32 + lane) / RC, c = (i * 32 + lane) % RC;
-                        const int t = __shfl_sync(0xffffffffu, tok, row), h = __shfl_sync(0xffffffffu, head, row);
+                        const int tr = __shfl_sync(0xffffffffu, t, row), h = __shfl_sync(0xffffffffu, head, row);
                         if (row < rows_left)
-                            *reinterpret_cast<uint4*>(p.out + ((size_t)(q0 + t) * p.nq + h) * D + (g * RC + c) * 8) =
+                            *reinterpret_cast<uint4*>(p.out + ((size_t)tr * p.nq + h) * D + (g * RC + c) * 8) =
                                 *reinterpret_cast<const uint4*>(cell(row, c));
                     }
                 } else {
+                    const int rows_left = left_of();
                     // slot 0 of the CTA: a piece of a walk that another one began; slot 1: of one that this one begins
-                    const size_t slot = ((size_t)blockIdx.x * 2 + (piece.at > 0 ? 0 : 1)) * ROWS + x * BLOCK_M + q * 32;
+                    const size_t slot = ((size_t)blockIdx.x * 2 + (now->p.at > 0 ? 0 : 1)) * ROWS + x * BLOCK_M + q * 32;
                     if (g == 0 && lane < rows_left)
-                        *reinterpret_cast<float2*>(p.part_ml + (slot + lane) * 2) = make_float2(m_used, rv ? l : 0.f);
-                    constexpr int W = D / 4;                       // columns at a time: 32 rows of them are what a warp's place holds
-                    auto cell = [&](int row, int c) { return rows + row * (W * 4) + ((c ^ (row & (W / 4 - 1))) << 4); };
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t v[W];
+                        *reinterpret_cast<float2*>(p.part_ml + (slot + lane) * 2) = make_float2(m_used, depth >= 0 ? l : 0.f);
+                    // four columns of a row at a time, those of all rows side by side: what 32 lanes write is one run
+                    float4* to = reinterpret_cast<float4*>(p.part_o) + (slot / ROWS) * (D / 4 * ROWS) + slot % ROWS + lane;
 #pragma unroll
-                        for (int c = 0; c < W / 16; ++c) tmem_ld16(t_o + g * (D / 2) + half * W + c * 16, v + c * 16);
+                    for (int c0 = 0; c0 < D / 8; c0 += 8) {
+                        uint32_t v[32];
+                        tmem_ld16(t_o + g * (D / 2) + c0 * 4, v);
+                        tmem_ld16(t_o + g * (D / 2) + c0 * 4 + 16, v + 16);
                         tmem_ld_wait();
+                        if (lane < rows_left) {
 #pragma unroll
-                        for (int c = 0; c < W / 4; ++c)
-                            *reinterpret_cast<uint4*>(cell(lane, c)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-                        __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < W / 4; ++i) {
-                            const int row = (i * 32 + lane) / (W / 4), c = (i * 32 + lane) % (W / 4);
-                            if (row < rows_left)
-                                *reinterpret_cast<uint4*>(p.part_o + (slot + row) * D + g * (D / 2) + half * W + c * 4) =
-                                    *reinterpret_cast<const uint4*>(cell(row, c));
+                            for (int c = 0; c < 8; ++c)
+                                to[(g * (D / 8) + c0 + c) * ROWS] = make_float4(__uint_as_float(v[4 * c]), __uint_as_float(v[4 * c + 1]),
+                                                                                __uint_as_float(v[4 * c + 2]), __uint_as_float(v[4 * c + 3]));
                         }
-                        __syncwarp();
                     }
                 }
             }
             tc_fence_before();
-            soft_sync();                                           // O, the queries' place and the parents may be written again
-            stage = (stage + nb) % NSTAGES;
+            soft_sync();                                           // O, the queries' place, the parents and the piece may be written again
         }
     }
     // ------------------------------------------------------------------ teardown
@@ -633,51 +684,69 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
     }
 }
 
-// Joins the pieces of the walks that are more than one share's: blocks (c, y) take JOIN_ROWS rows of the walk that ends in share c.
+// Joins the pieces of the walks that are more than one share's: a block takes JOIN_ROWS rows of the walk that ends in share
+// blockIdx.x; eight threads a row, each every eighth four of its columns.
 template <int D, int QT>
-__global__ void __launch_bounds__(128) attn_tree_join_kernel(const TreeTcParams p) {
-    constexpr int ROWS = QT * BLOCK_M, W = D / 4;
+__global__ void __launch_bounds__(JOIN_ROWS * 8) attn_tree_join_kernel(const TreeTcParams p) {
+    constexpr int ROWS = QT * BLOCK_M, FOURS = D / 32, AHEAD = 4;
     pdl_launch_dependents();
     pdl_wait();
     const int4 join = __ldcg(p.joins + blockIdx.x);                // request, kv head, tile, the first share
     if (join.x < 0) return;
-    const int G = p.nq / p.nkv, b = join.x, last = blockIdx.x;
-    const int q0 = p.q_start[b], rows_total = min(p.q_start[b + 1] - q0, TREE_MAX_NODES) * G;
-    for (int idx = threadIdx.x; idx < JOIN_ROWS * W; idx += 128) {
-        const int row = blockIdx.y * JOIN_ROWS + idx / W, c = idx % W;
-        const int R = join.z * ROWS + row;
-        if (R >= rows_total) return;
-        auto slot = [&](int s) { return ((size_t)s * 2 + (s == join.w ? 1 : 0)) * ROWS + row; };
-        float m = -INFINITY;
-#pragma unroll 4
-        for (int s = join.w; s <= last; ++s) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + slot(s));
-            if (ml.y > 0.f) m = fmaxf(m, ml.x);
+    const int b = join.x, last = blockIdx.x;
+    const int row = blockIdx.y * JOIN_ROWS + threadIdx.x / 8, c = threadIdx.x % 8, R = join.z * ROWS + row;
+    const int q0 = p.q_start[b], rows_total = min(p.q_start[b + 1] - q0, TREE_MAX_NODES) * p.group;
+    if (R >= rows_total) return;
+    float m = -INFINITY, l = 0.f;
+    float4 o[FOURS];
+#pragma unroll
+    for (int k = 0; k < FOURS; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = join.w; s0 <= last; s0 += AHEAD) {
+        float2 ml[AHEAD];
+        float4 v[AHEAD][FOURS];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int s = min(s0 + i, last);
+            const size_t slot = (size_t)s * 2 + (s == join.w ? 1 : 0);
+            ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + slot * ROWS + row);
+#pragma unroll
+            for (int k = 0; k < FOURS; ++k) v[i][k] = __ldcg(reinterpret_cast<const float4*>(p.part_o) + (slot * (D / 4) + k * 8 + c) * ROWS + row);
         }
-        const float ms = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int s = join.w; s <= last; ++s) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + slot(s));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot(s) * D) + c);
-            if (!(ml.y > 0.f)) continue;                           // a piece that the row saw nothing of counts for nothing
-            const float f = exp2f(ml.x - ms);
-            l = fmaf(ml.y, f, l);
-            o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+        // (a piece that the row saw nothing of counts for nothing)
+        float most = m;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) if (s0 + i <= last && ml[i].y > 0.f) most = fmaxf(most, ml[i].x);
+        const float f0 = m == -INFINITY ? 0.f : exp2f(m - most);
+        l *= f0;
+#pragma unroll
+        for (int k = 0; k < FOURS; ++k) { o[k].x *= f0; o[k].y *= f0; o[k].z *= f0; o[k].w *= f0; }
+        m = most;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (s0 + i > last || !(ml[i].y > 0.f)) continue;
+            const float f = exp2f(ml[i].x - m);
+            l = fmaf(ml[i].y, f, l);
+#pragma unroll
+            for (int k = 0; k < FOURS; ++k) {
+                o[k].x = fmaf(v[i][k].x, f, o[k].x); o[k].y = fmaf(v[i][k].y, f, o[k].y);
+                o[k].z = fmaf(v[i][k].z, f, o[k].z); o[k].w = fmaf(v[i][k].w, f, o[k].w);
+            }
         }
-        const int t = q0 + R / G, h = join.y * G + R % G;
-        float inv = 0.f;
-        if (l > 0.f) inv = (p.gate ? __ldcg(p.gate + (size_t)t * p.nq + h) : 1.f) / (p.sink ? l + exp2f(attn_sink_log2(p.sink_val, h) - ms) : l);
-        __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * inv, o.y * inv), hi = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+    }
+    const int tok = node_of(p, R), t = q0 + tok, h = join.y * p.group + (R - tok * p.group);
+    float inv = 0.f;
+    if (l > 0.f) inv = (p.gate ? __ldcg(p.gate + (size_t)t * p.nq + h) : 1.f) / (p.sink ? l + exp2f(attn_sink_log2(p.sink_val, h) - m) : l);
+#pragma unroll
+    for (int k = 0; k < FOURS; ++k) {
+        __nv_bfloat162 lo = __floats2bfloat162_rn(o[k].x * inv, o[k].y * inv), hi = __floats2bfloat162_rn(o[k].z * inv, o[k].w * inv);
         if (!(l > 0.f)) lo = hi = __floats2bfloat162_rn(0.f, 0.f);
-        *reinterpret_cast<uint2*>(p.out + ((size_t)t * p.nq + h) * D + c * 4) =
+        *reinterpret_cast<uint2*>(p.out + ((size_t)t * p.nq + h) * D + (k * 8 + c) * 4) =
             make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
     }
 }
 
 template <int D, int QT>
-int launch(const CUtensorMap& tm, const TreeTcParams& p, int ctas, bool join, cudaStream_t stream) {
+int launch(const CUtensorMap& tm, const TreeTcParams& p, int ctas, cudaStream_t stream) {
     constexpr int smem = TreeCfg<D, QT>::kSmem;
     auto kern = attn_tree_tc_kernel<D, QT>;
     static bool configured = false;
@@ -686,47 +755,46 @@ int launch(const CUtensorMap& tm, const TreeTcParams& p, int ctas, bool join, cu
         configured = true;
     }
     const int st = tff_launch_pdl(kern, dim3(ctas), dim3(TreeCfg<D, QT>::kThreads), (size_t)smem, stream, tm, p);
-    if (st != TFF_OK || !join) return st;
-    return tff_launch_pdl(attn_tree_join_kernel<D, QT>, dim3(ctas, QT * BLOCK_M / JOIN_ROWS), dim3(128), (size_t)0, stream, p);
+    if (st != TFF_OK || p.whole) return st;
+    return tff_launch_pdl(attn_tree_join_kernel<D, QT>, dim3(ctas, QT * BLOCK_M / JOIN_ROWS), dim3(JOIN_ROWS * 8), (size_t)0, stream, p);
 }
-
-int tiles_at_once(int max_nodes, int nq, int nkv) { return max_nodes * (nq / nkv) > BLOCK_M ? 2 : 1; }
 
 }  // namespace
 
-// Bytes of workspace of a call whose largest request brings max_nodes nodes.
-TFF_API long long tff_attention_tree_tc_workspace(int max_nodes, int nq, int nkv, int d) {
-    if (max_nodes <= 0 || nkv <= 0 || nq <= 0 || nq % nkv || d <= 0) return 0;
-    const long long rows = (long long)tff_num_sms() * 2 * tiles_at_once(max_nodes, nq, nkv) * BLOCK_M;
-    return rows * (d + 2) * 4 + (long long)tff_num_sms() * 16;
-}
-
-// TFF_ERR_UNSUPPORTED, with nothing launched, for what the general kernel (attention_tree.cu) has to take.
+// TFF_ERR_UNSUPPORTED, with nothing launched, for what the general kernel (attention_tree.cu) has to take.  A CTA's share has at least
+// ``least`` units, a walk ``extra`` of them ahead of its blocks; ``whole``: no walk is divided, and there is no second kernel.  ``ws``: an SM has 4 words and room for two pieces of 128 rows (256 where some request may have more rows
+// than 128) of d + 2 floats.
 TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* pos_start, const int* parents, const int* block_table,
                                   int table_width, const void* cache, long long cache_pages, int cache_layers, int layer, int page_size,
                                   void* out, int num_tokens, int requests, int max_nodes, int nq, int nkv, int d, float scale, int window,
-                                  float softcap, int sink, const float* sink_val, const float* gate, int keep, void* ws,
-                                  cudaStream_t stream) {
+                                  float softcap, int sink, const float* sink_val, const float* gate, int keep, int least, int extra, int whole, void* ws,
+                                  long long ws_floats, cudaStream_t stream) {
     if (num_tokens <= 0 || requests <= 0 || max_nodes <= 0) return TFF_OK;
     if (!q || !q_start || !pos_start || !parents || !block_table || !cache || !out || nq <= 0 || nkv <= 0 || nq % nkv || softcap < 0.f ||
-        keep < 0 || !ws)
+        keep < 0 || least <= 0 || extra < 0 || extra > 64 || table_width <= 0 || !ws)
         return TFF_ERR_BAD_ARGUMENT;
     if ((d != 64 && d != 128) || (page_size != 8 && page_size != 16 && page_size != 32 && page_size != 64)) return TFF_ERR_UNSUPPORTED;
+    if (nq / nkv > 255) return TFF_ERR_UNSUPPORTED;          // (a row's node by a product of 32 bits)
     if (cache_pages <= 0 || !(scale > 0.f) || max_nodes > TREE_MAX_NODES) return TFF_ERR_UNSUPPORTED;   // (a positive scale is folded into the exponent)
     if (((uintptr_t)cache & 15) || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || ((uintptr_t)ws & 15)) return TFF_ERR_UNSUPPORTED;
     const long long rows = cache_pages * cache_layers * 2 * nkv * page_size;
     const int sms = tff_num_sms();
     if (rows >= (1ll << 31) || sms <= 0) return TFF_ERR_UNSUPPORTED;
+    const int qt = (long long)max_nodes * (nq / nkv) > BLOCK_M ? 2 : 1;
+    // (the line's units are counted in 32 bits)
+    if ((((long long)table_width * page_size + TREE_MAX_NODES) / BLOCK_N + 2 + extra) * requests * nkv * ((long long)TREE_MAX_NODES * (nq / nkv) / BLOCK_M + 1) >= (1ll << 31))
+        return TFF_ERR_UNSUPPORTED;
+    if (ws_floats < (long long)sms * (4 + 2 * qt * BLOCK_M * (d + 2))) return TFF_ERR_BAD_ARGUMENT;
     CUtensorMap tm;
     if (!tff_tensor_map_kv_groups(cache, rows, d, page_size, nkv, &tm)) return TFF_ERR_DRIVER;
-    const int qt = tiles_at_once(max_nodes, nq, nkv);
     TreeTcParams p = {};
     p.q = (const bf16*)q; p.out = (bf16*)out;
     p.q_start = q_start; p.pos_start = pos_start; p.parents = parents; p.block_table = block_table;
     p.requests = requests; p.table_width = table_width; p.cache_layers = cache_layers; p.layer = layer;
     p.page_shift = page_size == 8 ? 3 : page_size == 16 ? 4 : page_size == 32 ? 5 : 6;
     p.nq = nq; p.nkv = nkv; p.window = window > 0 ? window : 0; p.keep = window > 0 ? keep : 0;
-    p.least = 4;
+    p.least = least; p.extra = extra; p.whole = whole;
+    p.group = nq / nkv; p.group_inverse = (unsigned)(((1ull << 32) + p.group - 1) / p.group);
     p.scale_log2 = scale * 1.4426950408889634f;
     p.scale_over_cap = softcap > 0.f ? scale / softcap : 0.f;
     p.cap_log2 = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
@@ -736,6 +804,6 @@ TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* 
     p.part_ml = p.part_o + (size_t)sms * 2 * qt * BLOCK_M * d;
     p.error_flag = tff_device_error_flag();
     if (p.error_flag == nullptr) return TFF_ERR_LAUNCH;
-    if (d == 128) return qt == 2 ? launch<128, 2>(tm, p, sms, true, stream) : launch<128, 1>(tm, p, sms, true, stream);
-    return qt == 2 ? launch<64, 2>(tm, p, sms, true, stream) : launch<64, 1>(tm, p, sms, true, stream);
+    if (d == 128) return qt == 2 ? launch<128, 2>(tm, p, sms, stream) : launch<128, 1>(tm, p, sms, stream);
+    return qt == 2 ? launch<64, 2>(tm, p, sms, stream) : launch<64, 1>(tm, p, sms, stream);
 }

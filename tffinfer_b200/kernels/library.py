@@ -183,13 +183,16 @@ class CudaKernels:
                 raise KernelError("kernels take contiguous tensors")
 
     @staticmethod
-    def _need_here(*tensors) -> None:
-        """_need_cuda, and on the current device, whose stream the launch goes to."""
-        CudaKernels._need_cuda(*tensors)
+    def _need_here(dtype, *tensors) -> None:
+        """Contiguous tensors of the type ``dtype`` (None: of any) on the current device, whose stream the launch goes to."""
         here = torch._C._cuda_getDevice()
         for t in tensors:
-            if t is not None and t.device.index != here:
-                raise KernelError(f"a tensor on cuda:{t.device.index} was given to a kernel on the current device, cuda:{here}")
+            if t is None or (t.get_device() == here and (dtype is None or t.dtype is dtype) and t.is_contiguous()):
+                continue
+            CudaKernels._need_cuda(t)
+            if t.get_device() != here:
+                raise KernelError(f"a tensor on cuda:{t.get_device()} was given to a kernel on the current device, cuda:{here}")
+            raise KernelError(f"a tensor of {t.dtype} where the kernel takes {dtype}")
 
     @staticmethod
     def _cache_args(kv_cache, kv_layer: int):
@@ -826,16 +829,16 @@ class CudaKernels:
                                        softcap, sink, gates, keep)
 
     TREE_MAX_NODES = 256          # of a request's tree of drafted tokens
+    TREE_WHOLE_BLOCKS = 8         # up to so many blocks of 64 keys a request's walk is not divided
 
-    def _tree_args(self, batch, parents, T: int) -> None:
-        """Checks what the kernels of drafted trees are given of a step."""
-        self._need_here(parents, batch.q_start, batch.pos_start)
-        B = batch.num_requests
-        if parents.dtype != torch.int32 or parents.numel() != T:
-            raise KernelError(f"parents are {T} int32 numbers, one a node")
-        if any(t.dtype != torch.int32 for t in (batch.q_start, batch.pos_start)) or batch.q_start.numel() < B + 1 or \
-                batch.pos_start.numel() < B:
-            raise KernelError("q_start and pos_start are int32, with an element a request (and one more)")
+    def _tree_args(self, batch, parents, T: int, *others) -> None:
+        """Checks what the kernels of drafted trees are given of a step, and ``others``, which are int32 as well."""
+        q_start, pos_start, B = batch.q_start, batch.pos_start, batch.num_requests
+        self._need_here(torch.int32, parents, q_start, pos_start, *others)
+        if parents.numel() != T:
+            raise KernelError(f"parents are {T} numbers, one a node")
+        if q_start.numel() <= B or pos_start.numel() < B:
+            raise KernelError("q_start and pos_start have an element a request, and q_start one more")
         if batch.max_q_len > self.TREE_MAX_NODES:
             raise KernelError(f"a request brings at most {self.TREE_MAX_NODES} nodes, got {batch.max_q_len}")
 
@@ -849,39 +852,56 @@ class CudaKernels:
         follows the cached tokens.  A node whose chain of parents does not end at -1 (padding: -2) sees nothing, is seen by
         none, and gives zeros.  A node's position, which counts for ``window`` and ``keep``, is pos_start[b] + its
         ancestors (the queries and keys are rotated by it: ``batch.positions`` of such a step).  At most 256 nodes a request."""
-        self._need_here(q, block_table, out, gates)
-        T, B = q.shape[0], batch.num_requests
+        T, B, dtype = q.shape[0], batch.num_requests, q.dtype
         dc = kv_cache.shape[-1]
-        if not (kv_cache.dtype == q.dtype == out.dtype) or kv_cache.device != q.device:
+        self._need_here(dtype, q, out)
+        self._tree_args(batch, parents, T, block_table)
+        if kv_cache.dtype is not dtype or kv_cache.get_device() != q.get_device():
             raise KernelError("queries, cache and outputs have one type and lie on one device")
-        if tuple(q.shape) != (T, nq * d) or tuple(out.shape) != (T, nq * dv) or tuple(kv_cache.shape[2:]) != (2, nkv, page_size, dc) \
-                or dc < max(d, dv):
+        if q.shape != (T, nq * d) or out.shape != (T, nq * dv) or kv_cache.shape[2:] != (2, nkv, page_size, dc) or dc < max(d, dv):
             raise KernelError("queries are [T, nq * d], outputs [T, nq * dv], cache pages [2, nkv, page, at least d and dv]")
-        if gates is not None and (gates.dtype != torch.float32 or tuple(gates.shape) != (T, nq)):
-            raise KernelError("head gates are float32 [T, nq]")
-        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < B:
-            raise KernelError("the block table is int32 [requests, pages]")
+        if gates is not None:
+            self._need_here(torch.float32, gates)
+            if gates.shape != (T, nq):
+                raise KernelError("head gates are [T, nq]")
+        if block_table.dim() != 2 or block_table.shape[0] < B:
+            raise KernelError("the block table is [requests, pages]")
         if not 0 <= kv_layer < kv_cache.shape[1]:
             raise KernelError(f"layer {kv_layer} of a cache of {kv_cache.shape[1]}")
-        self._tree_args(batch, parents, T)
         if T == 0 or B == 0:
             return
-        if q.dtype == torch.bfloat16 and d == dv == dc and d in (64, 128):
-            c_ptr, c_pages, c_layers, c_layer = self._cache_args(kv_cache, kv_layer)
-            sink_on, sink_val = self._sink_args(sink, nq)
-            ws = torch.empty(self.lib.tff_attention_tree_tc_workspace(_c_int(batch.max_q_len), _c_int(nq), _c_int(nkv), _c_int(d)),
-                             dtype=torch.uint8, device=q.device)
-            status = self.lib.tff_attention_tree_tc(
-                _ptr(q), _ptr(batch.q_start), _ptr(batch.pos_start), _ptr(parents), _ptr(block_table), _c_int(block_table.shape[1]),
-                c_ptr, _c_int(c_pages), _c_int(c_layers), _c_int(c_layer), _c_int(page_size), _ptr(out), _c_int(T), _c_int(B),
-                _c_int(batch.max_q_len), _c_int(nq), _c_int(nkv), _c_int(d), _c_float(scale), _c_int(window), _c_float(softcap),
-                _c_int(1 if sink_on else 0), _ptr(sink_val), _ptr(gates), _c_int(keep), _ptr(ws), self._stream())
-            if status != -2:                              # (what the kernel does not take, the general one does)
-                self._check(status, "attention_tree_tc")
-                self.launches += 2
-                return
+        if dtype is torch.bfloat16 and d == dv == dc and d in (64, 128) and \
+                self._attention_tree_tc(q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, scale, window,
+                                        softcap, sink, gates, keep):
+            return
         self._attention_tree_plain(q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window,
                                    softcap, sink, gates, keep)
+
+    def _attention_tree_tc(self, q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, scale, window,
+                           softcap, sink, gates, keep, least: int = 4, extra: int = 3, whole=None) -> bool:
+        """On the tensor cores; False, and nothing launched, for what that kernel does not take.  ``least``: blocks of 64 keys that
+        a CTA's share has at least; ``extra``: how many of them a piece of a walk costs beside its own; ``whole``: shares are whole walks (None: where none has more than WHOLE_BLOCKS)."""
+        T, B = q.shape[0], batch.num_requests
+        if whole is None:
+            keys = block_table.shape[1] * page_size if getattr(batch, "graph_bucket", None) is not None else int(batch.max_kv_len)
+            whole = min(keys, window + keep + batch.max_q_len if window > 0 else keys) <= self.TREE_WHOLE_BLOCKS * 64
+        c_ptr, c_pages, c_layers, c_layer = self._cache_args(kv_cache, kv_layer)
+        sink_on, sink_val = self._sink_args(sink, nq)
+        # a CTA's shares of two walks: rows of d values, a maximum and a sum; and which walk it ends
+        rows = 2 * self.NUM_SMS * (256 if batch.max_q_len * (nq // nkv) > 128 else 128)
+        ws = torch.empty(rows * (d + 2) + 4 * self.NUM_SMS, dtype=torch.float32, device=q.device)
+        status = self.lib.tff_attention_tree_tc(
+            _ptr(q), _ptr(batch.q_start), _ptr(batch.pos_start), _ptr(parents), _ptr(block_table), _c_int(block_table.shape[1]),
+            c_ptr, _c_int(c_pages), _c_int(c_layers), _c_int(c_layer), _c_int(page_size), _ptr(out), _c_int(T), _c_int(B),
+            _c_int(batch.max_q_len), _c_int(nq), _c_int(nkv), _c_int(d), _c_float(scale), _c_int(window), _c_float(softcap),
+            _c_int(1 if sink_on else 0), _ptr(sink_val), _ptr(gates), _c_int(keep), _c_int(least), _c_int(extra), _c_int(1 if whole else 0), _ptr(ws),
+            _c_int(ws.numel()),
+            self._stream())
+        if status == -2:
+            return False
+        self._check(status, "attention_tree_tc")
+        self.launches += 1 if whole else 2
+        return True
 
     def _attention_tree_plain(self, q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window,
                               softcap, sink, gates, keep, splits=None) -> None:
@@ -910,10 +930,7 @@ class CudaKernels:
         both -1 beyond; count int32 [B]: their number (0 for a request without nodes)."""
         tokens = batch.token_ids
         T, B = tokens.numel(), batch.num_requests
-        self._need_here(tokens, drawn, path, emitted, count)
-        self._tree_args(batch, parents, T)
-        if any(t.dtype != torch.int32 for t in (tokens, drawn, path, emitted, count)):
-            raise KernelError("tokens, paths and counts are int32")
+        self._tree_args(batch, parents, T, tokens, drawn, path, emitted, count)
         if drawn.numel() != T or path.dim() != 2 or path.shape[0] != B or path.shape != emitted.shape or count.numel() != B:
             raise KernelError("a draw a node, and path and emitted [requests, width], count [requests]")
         if B == 0 or path.shape[1] == 0:
@@ -928,13 +945,11 @@ class CudaKernels:
         """The keys and values of the accepted nodes go to where the next step expects them, in every layer of the cache
         [pages, layers, planes, kv heads, page, head]: slot pos_start[b] + path[b, j] to slot pos_start[b] + j, j < count[b].
         path and count as ``accept_tree`` gives them (a path's nodes ascend); the slots behind stay as they are."""
-        self._need_here(block_table, path, count, batch.pos_start)
         B = batch.num_requests
-        if any(t.dtype != torch.int32 for t in (block_table, path, count, batch.pos_start)):
-            raise KernelError("block table, paths, counts and positions are int32")
+        self._need_here(torch.int32, block_table, path, count, batch.pos_start)
         if kv_cache.dim() != 6 or kv_cache.shape[4] != page_size:
             raise KernelError("the cache is [pages, layers, planes, kv heads, page, head]")
-        if kv_cache.device != path.device:
+        if kv_cache.get_device() != path.get_device():
             raise KernelError("the cache is on another device")
         if path.dim() != 2 or path.shape[0] != B or count.numel() != B or block_table.dim() != 2 or block_table.shape[0] < B or \
                 batch.pos_start.numel() < B:
@@ -2383,11 +2398,12 @@ class CudaKernels:
         """out = logits (float32 [R, V]) under ``controls`` (sampling.LogitControls): penalties for repeated tokens, biases,
         grammar masks.  ``out`` may be ``logits`` itself unless the rows are nodes of trees."""
         c = controls
-        self._need_here(logits, out, c.row_start, c.settings, c.history, c.history_start, c.history_len, c.prompt_len, c.bias_start,
-                        c.bias_tokens, c.bias_values, c.mask, c.mask_row, c.parents, c.tokens)
+        self._need_here(torch.float32, logits, out, c.settings, c.bias_values)
+        self._need_here(torch.int32, c.row_start, c.history, c.history_start, c.history_len, c.prompt_len, c.bias_start, c.bias_tokens,
+                        c.mask, c.mask_row, c.parents, c.tokens)
         R, V = logits.shape
-        if logits.dtype != torch.float32 or out.dtype != torch.float32 or out.shape != logits.shape:
-            raise KernelError("logits and outputs are float32 [rows, vocabulary]")
+        if out.shape != logits.shape:
+            raise KernelError("logits and outputs are [rows, vocabulary]")
         problem = c.problem(R, V)
         if problem is not None:
             raise KernelError(f"logit controls: {problem}")

@@ -5,7 +5,7 @@ called.  Here the rows of a whole step, single tokens or the nodes of drafted tr
 (``CudaKernels.control_logits``)."""
 from __future__ import annotations
 
-from dataclasses import dataclass, fields
+from dataclasses import dataclass
 from typing import Optional, Sequence
 
 import numpy as np
@@ -52,37 +52,30 @@ class LogitControls:
     parents: Optional[torch.Tensor] = None
     tokens: Optional[torch.Tensor] = None
 
-    FLOATS = ("settings", "bias_values")
-
     def problem(self, rows: int, vocab: int) -> Optional[str]:
-        """What is wrong with these controls for logits [rows, vocab], or None."""
-        for f in fields(self):
-            t = getattr(self, f.name)
-            if t is None:
-                continue
-            want = torch.float32 if f.name in self.FLOATS else torch.int32
-            if t.dtype != want:
-                return f"{f.name} is {t.dtype}, not {want}"
+        """What is wrong with the sizes of these controls for logits [rows, vocab], or None."""
         B = self.row_start.numel() - 1
-        if B < 0 or tuple(self.settings.shape) != (B, 3):
+        if B < 0 or self.settings.shape != (B, 3):
             return "row_start has one element more than settings has rows of three"
-        if any(t.numel() != B for t in (self.history_start, self.history_len, self.prompt_len)):
+        if self.history_start.numel() != B or self.history_len.numel() != B or self.prompt_len.numel() != B:
             return "history_start, history_len and prompt_len have an element a request"
-        biases = (self.bias_start, self.bias_tokens, self.bias_values)
-        if any(t is None for t in biases) != all(t is None for t in biases):
-            return "bias_start, bias_tokens and bias_values come together"
-        if self.bias_start is not None and (self.bias_start.numel() != B + 1 or self.bias_tokens.numel() != self.bias_values.numel()):
-            return "bias_start has an element more than there are requests, bias_tokens as many as bias_values"
-        if self.mask is not None and (self.mask.dim() != 2 or self.mask.shape[1] * 32 < vocab):
-            return f"a mask has a bit for each of {vocab} tokens"
-        if self.mask is None and self.mask_row is not None:
+        if self.bias_start is not None or self.bias_tokens is not None or self.bias_values is not None:
+            if self.bias_start is None or self.bias_tokens is None or self.bias_values is None:
+                return "bias_start, bias_tokens and bias_values come together"
+            if self.bias_start.numel() != B + 1 or self.bias_tokens.numel() != self.bias_values.numel():
+                return "bias_start has an element more than there are requests, bias_tokens as many as bias_values"
+        if self.mask is not None:
+            if self.mask.dim() != 2 or self.mask.shape[1] * 32 < vocab:
+                return f"a mask has a bit for each of {vocab} tokens"
+        elif self.mask_row is not None:
             return "mask_row without a mask"
         if self.mask_row is not None and self.mask_row.numel() != rows:
             return "mask_row has an element a row"
-        if (self.parents is None) != (self.tokens is None):
-            return "parents and tokens come together"
-        if self.parents is not None and (self.parents.numel() != rows or self.tokens.numel() != rows):
-            return "parents and tokens have an element a row"
+        if self.parents is not None or self.tokens is not None:
+            if self.parents is None or self.tokens is None:
+                return "parents and tokens come together"
+            if self.parents.numel() != rows or self.tokens.numel() != rows:
+                return "parents and tokens have an element a row"
         return None
 
     @classmethod
