@@ -43,14 +43,15 @@ using tc5::tc_fence_after;
 using tc5::tmem_ld16;
 using tc5::tmem_ld_wait;
 
-constexpr int BLOCK_M = 128, BLOCK_N = 64, BARS_PER_TILE = 16, JOIN_ROWS = 32;
+constexpr int BLOCK_M = 128, BLOCK_N = 64, BARS_PER_TILE = 17, JOIN_ROWS = 32;
 constexpr float RESCALE_THRESHOLD = 8.0f;            // in log2 units
 
 struct TreeTcParams {
-    const bf16* q; bf16* out;
+    bf16* out;
     const int *q_start, *pos_start, *parents, *block_table;
     int requests, table_width, cache_layers, layer, page_shift, nq, nkv, window, keep, least, extra, whole;
     int group; unsigned group_inverse;               // query heads a kv head, and what a row number is multiplied by for its node
+    int tile_rows;                                   // of 128: whole nodes
     float scale_log2, scale_over_cap, cap_log2;
     int sink; const float *sink_val, *gate;
     float *part_o, *part_ml; int4* joins;
@@ -64,6 +65,13 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* tm,
         ::"r"(dst), "l"(tm), "r"(bar), "r"(0), "r"(group) : "memory");
 }
 
+// A box of tff_tensor_map_heads: 64 columns (of a half) of the heads of a group, of a tile's nodes.
+__device__ __forceinline__ void tma_load_queries(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int half, int kvh, int token) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %3, %4, %5, %6}], [%2];"
+        ::"r"(dst), "l"(tm), "r"(bar), "r"(0), "r"(half), "r"(kvh), "r"(token) : "memory");
+}
+
 template <int D, int QT>
 struct TreeCfg {
     static constexpr int kQBytes = BLOCK_M * D * 2;                 // [64-column half][128 rows][128 B]
@@ -72,7 +80,7 @@ struct TreeCfg {
     static constexpr int kExchange = QT * 2 * BLOCK_M * 4;          // a float of every row from either group
     static constexpr int kParents = TREE_MAX_NODES * 2;
     static constexpr int kBars = 2 * kStages + BARS_PER_TILE * QT;
-    static constexpr int kSmem = QT * kQBytes + kStages * kStageBytes + kExchange + kParents + 8 * kBars + 8 + 2 * 80;
+    static constexpr int kSmem = QT * kQBytes + kStages * kStageBytes + kExchange + kParents + 8 * kBars + 8 + 2 * 76;
     static constexpr int kThreads = (8 * QT + 1 + QT) * 32;
     static_assert(kSmem <= 227 * 1024, "shared memory of the tree attention kernel");
 };
@@ -115,13 +123,12 @@ struct Pieces {
     int unit = 0;                                    // of the walk, behind the present piece
     Walk w;
     // A warp's, with all its lanes; returns the line's units and the share's first one.
-    template <int ROWS>
-    __device__ __forceinline__ int2 start(const TreeTcParams& p) {
+    __device__ __forceinline__ int2 start(const TreeTcParams& p, int rows) {
         const int lane = threadIdx.x & 31;
         Walk v;
         auto sum_of = [&](int r0) -> int {           // inclusive sums of 32 requests' units
             v = Walk();
-            if (r0 + lane < p.requests) v.read(p, r0 + lane, ROWS);
+            if (r0 + lane < p.requests) v.read(p, r0 + lane, rows);
             int s = v.count > 0 ? v.tiles * (v.count + p.extra) : 0;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
@@ -165,8 +172,7 @@ struct Pieces {
         return make_int2(line * p.nkv, first);
     }
     // The next piece; false behind the last.
-    template <int ROWS>
-    __device__ __forceinline__ bool next(const TreeTcParams& p) {
+    __device__ __forceinline__ bool next(const TreeTcParams& p, int rows) {
         if (left <= 0) return false;
         if (unit == w.count + p.extra) {
             unit = 0;
@@ -174,7 +180,7 @@ struct Pieces {
                 tile = 0;
                 do {
                     if (++b == p.requests) { b = 0; ++kvh; }
-                    w.read(p, b, ROWS);
+                    w.read(p, b, rows);
                 } while (w.count == 0);
             }
         }
@@ -204,13 +210,13 @@ __device__ __forceinline__ uint64_t below(int k) { return k <= 0 ? 0ull : k >= 6
 // QT: query tiles a CTA walks with at once, two where some request has more rows than one.
 template <int D, int QT>
 __global__ void __launch_bounds__(TreeCfg<D, QT>::kThreads, 1)
-attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcParams p) {
+attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const __grid_constant__ CUtensorMap tm_q, const TreeTcParams p) {
     using Cfg = TreeCfg<D, QT>;
     constexpr int HALVES = D / 64, CH = D / 8;                   // 64-column halves, 16-byte chunks of a key or value row
     constexpr int NSTAGES = Cfg::kStages, STAGE_BYTES = Cfg::kStageBytes;
     constexpr int GROUP = 2 * HALVES * 1024;                     // of a stage, [8 keys][K, V][half]: from 8 keys to the next 8
     constexpr int V_AT = HALVES * 1024;
-    constexpr int ROWS = QT * BLOCK_M, SOFT = QT * 256;          // rows of a piece, softmax threads
+    constexpr int ROWS = QT * BLOCK_M, SOFT = QT * 256;          // places of a piece's rows, softmax threads
     constexpr int TMEM_COLS = 512;                               // all of it: the allocation starts at column 0
     constexpr int LOAD_WARP = 8 * QT, ISSUE_WARP = LOAD_WARP + 1;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -230,12 +236,13 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
     auto pv_done = [&](int x, int g) { return tile_bar(x, 5 + g); };
     auto q_ready = [&](int x) { return tile_bar(x, 7); };
     auto ref_bar = [&](int x, int g, int q) { return tile_bar(x, 8 + 4 * g + q); };
+    auto q_free = [&](int x) { return tile_bar(x, 16); };
     volatile uint32_t* tmem_slot = (volatile uint32_t*)(smem + BARS_AT + 8 * Cfg::kBars);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     Present* present = (Present*)(tmem_slot + 2);                // [2]: the piece, and the next one
-    static_assert(sizeof(Present) <= 80, "a piece's place");
+    static_assert(sizeof(Present) <= 76, "a piece's place");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int G = p.group;
+    const int G = p.group, rows = QT * p.tile_rows;
 
     if (tid == 0) {
         for (int s = 0; s < NSTAGES; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), QT); }
@@ -244,11 +251,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                 mbar_init(s_full(x, g), 1); mbar_init(p_full(x, g), 4); mbar_init(pv_done(x, g), 1);
                 for (int q = 0; q < 4; ++q) mbar_init(ref_bar(x, g, q), 1);
             }
-            mbar_init(s_free(x), 4); mbar_init(q_ready(x), 8);
+            mbar_init(s_free(x), 4); mbar_init(q_ready(x), 1); mbar_init(q_free(x), 1);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_cache) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_q) : "memory");
     }
     if (warp == ISSUE_WARP) tmem_alloc(smem_u32((const void*)tmem_slot), TMEM_COLS);
     tc_fence_before();
@@ -257,8 +265,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
     constexpr uint32_t tmem_base = 0;
     pdl_launch_dependents();
     pdl_wait();
-    Pieces piece;
-    const int2 line = piece.template start<ROWS>(p);
+    Pieces piece;                                                // (the other softmax warps read it from shared memory)
+    int2 line = make_int2(0, 0);
+    if (warp == 0 || warp >= LOAD_WARP) line = piece.start(p, rows);
 
     if (warp == LOAD_WARP) {
         // ------------------------------------------------------------ TMA producer
@@ -273,7 +282,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
         int s = 0;
         uint32_t round = 0;
         bool ok = true;
-        while (ok && piece.template next<ROWS>(p)) {
+        while (ok && piece.next(p, rows)) {
             const KeyWalk walk = piece.w.keys(p.keep);
             const int* table = p.block_table + (size_t)piece.b * p.table_width;
             const int table_end = piece.w.hi() >> p.page_shift;
@@ -323,8 +332,8 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
             uint32_t phase = 0, phase_q = 0, phase_s = 1;          // of the ring, the queries, s_free (nothing to wait for at first)
             uint32_t phase_p[2] = {0, 0};
             int st = 0, st_pv = 0;                                 // stages of S(n) and of PV(n - 2)
-            while (ok && piece.template next<ROWS>(p)) {
-                if (piece.tile * ROWS + x * BLOCK_M >= piece.w.nodes * G) {
+            while (ok && piece.next(p, rows)) {
+                if (piece.tile * rows + x * p.tile_rows >= piece.w.nodes * G) {
                     // a tile without rows gives the stages back as they arrive
                     for (int n = 0; n < piece.nb && ok; ++n) {
                         ok = mbar_wait_warp(kv_full(st), phase, abort_flag);
@@ -335,6 +344,18 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                     st_pv = st;
                     continue;
                 }
+                // the queries, once the products of the piece before have read theirs; padding and rows of other requests among them
+                // make rows of their own, which are not stored
+                ok = mbar_wait_warp(q_free(x), phase_q ^ 1, abort_flag);
+                if (!ok) break;
+                if (lane == 0) {
+                    mbar_expect_tx(q_ready(x), (uint32_t)(HALVES * p.tile_rows * 128));
+                    const int token = piece.w.q0 + (piece.tile * QT + x) * (p.tile_rows / G);
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h)
+                        tma_load_queries(sQ + x * Cfg::kQBytes + h * (BLOCK_M * 128), &tm_q, q_ready(x), h, piece.kvh, token);
+                }
+                __syncwarp();
                 ok = mbar_wait_warp(q_ready(x), phase_q, abort_flag);
                 phase_q ^= 1;
                 // S runs two blocks ahead of PV: a group that has written P(j) finds S(j + 2) finished
@@ -350,6 +371,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                         for (int h = 0; h < HALVES; ++h)
                             umma4_bf16_elected(t_s, qdesc + (uint64_t)(h * (BLOCK_M * 128) >> 4), kd + (uint64_t)(h * 1024 >> 4), idesc_s, h > 0 ? 1u : 0u);
                         umma_commit_elected(s_full(x, n & 1));
+                        if (n == piece.nb - 1) umma_commit_elected(q_free(x));
                         if (++st == NSTAGES) { st = 0; phase ^= 1; }
                     }
                     const int j = n - 2;
@@ -386,7 +408,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
         uint32_t n_own = 0, n_other = 0;
         bool ok = true;
         if (tid == 0) {
-            present->go = piece.template next<ROWS>(p);
+            present->go = piece.next(p, rows);
             present->p = piece;
             present->keys = piece.w.keys(p.keep);
             present->stage = 0;
@@ -395,46 +417,19 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
         soft_sync();
         for (const Present* now = present;; now = present + (now == present)) {
             if (!now->go) break;
-            const int rows_total = now->p.w.nodes * G;
-            auto row_of = [&]() { return now->p.tile * ROWS + x * BLOCK_M + r; };
-            auto left_of = [&]() { return min(32, now->p.w.nodes * G - (row_of() - lane)); };      // rows of this warp's 32 that exist
-            const int R = row_of(), rows_left = left_of(), tok = node_of(p, R);
-            const bool tile_active = R - r < rows_total;
-            // ---------------------------------- queries and parents; half of the columns of this warp's rows a group
-            constexpr int RC = D / 16;                             // 16-byte chunks of a row that a group has
-            uint4 u[RC];
-            if (rows_left > 0) {
-                // (rows that do not exist take the last one's place: no load waits for another)
-                const bf16* from = p.q + ((size_t)now->p.w.q0 * p.nq + now->p.kvh * G) * D + g * RC * 8;
-#pragma unroll
-                for (int i = 0; i < RC; ++i) {
-                    const int row = min((i * 32 + lane) / RC, rows_left - 1), c = (i * 32 + lane) % RC;
-                    const int of = R - lane + row, t = node_of(p, of);
-                    u[i] = __ldcg(reinterpret_cast<const uint4*>(from + ((size_t)t * p.nq + (of - t * G)) * D + c * 8));
-                }
-            }
+            auto row_of = [&]() { return (now->p.tile * QT + x) * p.tile_rows + r; };
+            auto exists = [&]() { return r < p.tile_rows && row_of() < now->p.w.nodes * G; };
+            const int tok = node_of(p, row_of());
+            const bool tile_active = row_of() - r < now->p.w.nodes * G;
             if (now->fresh) {
                 const int nodes = now->p.w.nodes;
                 for (int i = tid; i < nodes; i += SOFT) parent[i] = tree_parent(__ldcg(p.parents + now->p.w.q0 + i), i);
                 soft_sync();
             }
-            const int depth = R < rows_total ? tree_depth(parent, tok) : -1;   // (-1: a row of no node that is there)
-            if (tile_active) {
-                uint8_t* dst = smem + x * Cfg::kQBytes + q * 32 * 128;
-#pragma unroll
-                for (int i = 0; i < RC; ++i) {
-                    const int row = (i * 32 + lane) / RC, c = g * RC + (i * 32 + lane) % RC;
-                    // padding has queries of zeros: whatever it brought, its scores are finite
-                    if (__shfl_sync(0xffffffffu, depth, row) < 0) u[i] = make_uint4(0u, 0u, 0u, 0u);
-                    *reinterpret_cast<uint4*>(dst + (c >> 3) * (BLOCK_M * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = u[i];
-                }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_ready(x));
-            }
+            const int depth = exists() ? tree_depth(parent, tok) : -1;         // (-1: a row of no node that is there)
             if (warp == 0) {                                       // the next piece, while the first products run
                 Pieces next = now->p;
-                const bool go = next.template next<ROWS>(p);
+                const bool go = next.next(p, rows);
                 Present* to = present + (now == present);
                 if (lane == 0) {
                     to->fresh = next.b != now->p.b;
@@ -445,16 +440,18 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                 }
                 __syncwarp();
             }
+            const int tail = now->p.w.ctx - BLOCK_N;               // blocks that begin behind it hold nodes
+            int n_first = (now->p.at + g) * BLOCK_N;
             float m_used = -INFINITY, l = 0.f;
             const int nb_x = tile_active ? now->p.nb : 0;
-            for (int j = g; j < nb_x && ok; j += 2) {
+            for (int j = g; j < nb_x && ok; j += 2, n_first += 2 * BLOCK_N) {
                 ok = mbar_wait_warp(s_full(x, g), n_own, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                const int n_first = now->keys.block(now->p.at + j) * BLOCK_N;
+                if (p.window > 0) n_first = now->keys.block(now->p.at + j) * BLOCK_N;
                 // Masked or capped scores are written back over the raw ones, so that the pass below is the same for every block.
                 // Rows that are not there are not stored: they need no mask.
-                const bool some_nodes = n_first + BLOCK_N > now->p.w.ctx;
+                const bool some_nodes = n_first > tail;
                 bool masked = some_nodes;
                 if (p.window > 0 && !some_nodes)
                     masked = !__all_sync(0xffffffffu, depth < 0 || n_first > now->p.w.ctx + depth - p.window || n_first + BLOCK_N <= p.keep);
@@ -517,7 +514,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                     if (!ok) break;
                     tc_fence_after();
                 }
-                if (some_nodes || now->keys.ragged(now->p.at + j)) {
+                if (some_nodes || (p.window > 0 && now->keys.ragged(now->p.at + j))) {      // (the last block holds nodes)
                     // value rows that no row may see (behind the last node, between the kept ones and the first window, of
                     // padding) are cleared, since slots and unfetched shared memory may hold anything; the warps of both tiles
                     // do it (the same zeros), so that each tile's products wait for its own warps only
@@ -607,21 +604,20 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
             l = g == 0 ? l + *other : *other + l;
             if (ok && nb_x > 0) {
                 tc_fence_after();
-                // through shared memory, where the queries lay (every S is finished), 32 rows a warp
-                uint8_t* rows = smem + x * Cfg::kQBytes + (g * 4 + q) * (32 * D);
                 if (now->p.all()) {
-                    const int rows_left = left_of(), t = now->p.w.q0 + tok, head = now->p.kvh * G + (row_of() - tok * G);
+                    const int t = now->p.w.q0 + tok, head = now->p.kvh * G + (row_of() - tok * G);
                     if (p.sink && l > 0.f) l += exp2f(attn_sink_log2(p.sink_val, head) - m_used);       // a key without a value
-                    const bool some = depth >= 0 && l > 0.f;               // (a padding row's sums may be anything)
+                    const bool some = depth >= 0 && l > 0.f;       // (a padding row's sums may be anything)
                     float inv = some ? 1.f / l : 0.f;
                     if (p.gate && some) inv *= __ldcg(p.gate + (size_t)t * p.nq + head);
-                    auto cell = [&](int row, int c) { return rows + row * D + ((c ^ (RC == 8 ? row & 7 : (row >> 1) & 3)) << 4); };
+                    uint4* to = reinterpret_cast<uint4*>(p.out + ((size_t)t * p.nq + head) * D + g * (D / 2));
 #pragma unroll
-                    for (int half = 0; half < RC / 4; ++half) {
+                    for (int c0 = 0; c0 < D / 2; c0 += 32) {
                         uint32_t v[32];
-                        tmem_ld16(t_o + g * (D / 2) + half * 32, v);
-                        tmem_ld16(t_o + g * (D / 2) + half * 32 + 16, v + 16);
+                        tmem_ld16(t_o + g * (D / 2) + c0, v);
+                        tmem_ld16(t_o + g * (D / 2) + c0 + 16, v + 16);
                         tmem_ld_wait();
+                        if (!exists()) continue;
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
                             uint32_t wd[4];
@@ -630,23 +626,13 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                                 __nv_bfloat162 b2 = __floats2bfloat162_rn(__uint_as_float(v[8 * c + 2 * i]) * inv, __uint_as_float(v[8 * c + 2 * i + 1]) * inv);
                                 wd[i] = some ? *reinterpret_cast<uint32_t*>(&b2) : 0u;
                             }
-                            *reinterpret_cast<uint4*>(cell(lane, half * 4 + c)) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+                            to[c0 / 8 + c] = make_uint4(wd[0], wd[1], wd[2], wd[3]);
                         }
                     }
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < RC; ++i) {
-                        const int row = (i * 32 + lane) / RC, c = (i * 32 + lane) % RC;
-                        const int tr = __shfl_sync(0xffffffffu, t, row), h = __shfl_sync(0xffffffffu, head, row);
-                        if (row < rows_left)
-                            *reinterpret_cast<uint4*>(p.out + ((size_t)tr * p.nq + h) * D + (g * RC + c) * 8) =
-                                *reinterpret_cast<const uint4*>(cell(row, c));
-                    }
                 } else {
-                    const int rows_left = left_of();
                     // slot 0 of the CTA: a piece of a walk that another one began; slot 1: of one that this one begins
                     const size_t slot = ((size_t)blockIdx.x * 2 + (now->p.at > 0 ? 0 : 1)) * ROWS + x * BLOCK_M + q * 32;
-                    if (g == 0 && lane < rows_left)
+                    if (g == 0 && exists())
                         *reinterpret_cast<float2*>(p.part_ml + (slot + lane) * 2) = make_float2(m_used, depth >= 0 ? l : 0.f);
                     // four columns of a row at a time, those of all rows side by side: what 32 lanes write is one run
                     float4* to = reinterpret_cast<float4*>(p.part_o) + (slot / ROWS) * (D / 4 * ROWS) + slot % ROWS + lane;
@@ -656,7 +642,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                         tmem_ld16(t_o + g * (D / 2) + c0 * 4, v);
                         tmem_ld16(t_o + g * (D / 2) + c0 * 4 + 16, v + 16);
                         tmem_ld_wait();
-                        if (lane < rows_left) {
+                        if (exists()) {
 #pragma unroll
                             for (int c = 0; c < 8; ++c)
                                 to[(g * (D / 8) + c0 + c) * ROWS] = make_float4(__uint_as_float(v[4 * c]), __uint_as_float(v[4 * c + 1]),
@@ -666,7 +652,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const TreeTcPa
                 }
             }
             tc_fence_before();
-            soft_sync();                                           // O, the queries' place, the parents and the piece may be written again
+            soft_sync();                                           // O, the parents and the piece may be written again
         }
     }
     // ------------------------------------------------------------------ teardown
@@ -694,9 +680,10 @@ __global__ void __launch_bounds__(JOIN_ROWS * 8) attn_tree_join_kernel(const Tre
     const int4 join = __ldcg(p.joins + blockIdx.x);                // request, kv head, tile, the first share
     if (join.x < 0) return;
     const int b = join.x, last = blockIdx.x;
-    const int row = blockIdx.y * JOIN_ROWS + threadIdx.x / 8, c = threadIdx.x % 8, R = join.z * ROWS + row;
+    const int row = blockIdx.y * JOIN_ROWS + threadIdx.x / 8, c = threadIdx.x % 8;
+    const int R = (join.z * QT + row / BLOCK_M) * p.tile_rows + row % BLOCK_M;
     const int q0 = p.q_start[b], rows_total = min(p.q_start[b + 1] - q0, TREE_MAX_NODES) * p.group;
-    if (R >= rows_total) return;
+    if (row % BLOCK_M >= p.tile_rows || R >= rows_total) return;
     float m = -INFINITY, l = 0.f;
     float4 o[FOURS];
 #pragma unroll
@@ -746,7 +733,7 @@ __global__ void __launch_bounds__(JOIN_ROWS * 8) attn_tree_join_kernel(const Tre
 }
 
 template <int D, int QT>
-int launch(const CUtensorMap& tm, const TreeTcParams& p, int ctas, cudaStream_t stream) {
+int launch(const CUtensorMap& tm, const CUtensorMap& tq, const TreeTcParams& p, int ctas, cudaStream_t stream) {
     constexpr int smem = TreeCfg<D, QT>::kSmem;
     auto kern = attn_tree_tc_kernel<D, QT>;
     static bool configured = false;
@@ -754,7 +741,7 @@ int launch(const CUtensorMap& tm, const TreeTcParams& p, int ctas, cudaStream_t 
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return TFF_ERR_LAUNCH;
         configured = true;
     }
-    const int st = tff_launch_pdl(kern, dim3(ctas), dim3(TreeCfg<D, QT>::kThreads), (size_t)smem, stream, tm, p);
+    const int st = tff_launch_pdl(kern, dim3(ctas), dim3(TreeCfg<D, QT>::kThreads), (size_t)smem, stream, tm, tq, p);
     if (st != TFF_OK || p.whole) return st;
     return tff_launch_pdl(attn_tree_join_kernel<D, QT>, dim3(ctas, QT * BLOCK_M / JOIN_ROWS), dim3(JOIN_ROWS * 8), (size_t)0, stream, p);
 }
@@ -774,27 +761,29 @@ TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* 
         keep < 0 || least <= 0 || extra < 0 || extra > 64 || table_width <= 0 || !ws)
         return TFF_ERR_BAD_ARGUMENT;
     if ((d != 64 && d != 128) || (page_size != 8 && page_size != 16 && page_size != 32 && page_size != 64)) return TFF_ERR_UNSUPPORTED;
-    if (nq / nkv > 255) return TFF_ERR_UNSUPPORTED;          // (a row's node by a product of 32 bits)
+    if (nq / nkv > BLOCK_M) return TFF_ERR_UNSUPPORTED;          // a tile holds whole nodes
     if (cache_pages <= 0 || !(scale > 0.f) || max_nodes > TREE_MAX_NODES) return TFF_ERR_UNSUPPORTED;   // (a positive scale is folded into the exponent)
     if (((uintptr_t)cache & 15) || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || ((uintptr_t)ws & 15)) return TFF_ERR_UNSUPPORTED;
     const long long rows = cache_pages * cache_layers * 2 * nkv * page_size;
     const int sms = tff_num_sms();
     if (rows >= (1ll << 31) || sms <= 0) return TFF_ERR_UNSUPPORTED;
-    const int qt = (long long)max_nodes * (nq / nkv) > BLOCK_M ? 2 : 1;
+    const int group = nq / nkv, tile_rows = BLOCK_M / group * group;
+    const int qt = (long long)max_nodes * group > tile_rows ? 2 : 1;
     // (the line's units are counted in 32 bits)
-    if ((((long long)table_width * page_size + TREE_MAX_NODES) / BLOCK_N + 2 + extra) * requests * nkv * ((long long)TREE_MAX_NODES * (nq / nkv) / BLOCK_M + 1) >= (1ll << 31))
+    if ((((long long)table_width * page_size + TREE_MAX_NODES) / BLOCK_N + 2 + extra) * requests * nkv * ((long long)TREE_MAX_NODES * group / tile_rows + 1) >= (1ll << 31))
         return TFF_ERR_UNSUPPORTED;
     if (ws_floats < (long long)sms * (4 + 2 * qt * BLOCK_M * (d + 2))) return TFF_ERR_BAD_ARGUMENT;
-    CUtensorMap tm;
+    CUtensorMap tm, tq;
     if (!tff_tensor_map_kv_groups(cache, rows, d, page_size, nkv, &tm)) return TFF_ERR_DRIVER;
+    if (!tff_tensor_map_heads(q, num_tokens, nkv, group, d, tile_rows / group, &tq)) return TFF_ERR_DRIVER;
     TreeTcParams p = {};
-    p.q = (const bf16*)q; p.out = (bf16*)out;
+    p.out = (bf16*)out;
     p.q_start = q_start; p.pos_start = pos_start; p.parents = parents; p.block_table = block_table;
     p.requests = requests; p.table_width = table_width; p.cache_layers = cache_layers; p.layer = layer;
     p.page_shift = page_size == 8 ? 3 : page_size == 16 ? 4 : page_size == 32 ? 5 : 6;
     p.nq = nq; p.nkv = nkv; p.window = window > 0 ? window : 0; p.keep = window > 0 ? keep : 0;
     p.least = least; p.extra = extra; p.whole = whole;
-    p.group = nq / nkv; p.group_inverse = (unsigned)(((1ull << 32) + p.group - 1) / p.group);
+    p.group = group; p.tile_rows = tile_rows; p.group_inverse = (unsigned)(((1ull << 32) + p.group - 1) / p.group);
     p.scale_log2 = scale * 1.4426950408889634f;
     p.scale_over_cap = softcap > 0.f ? scale / softcap : 0.f;
     p.cap_log2 = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
@@ -804,6 +793,6 @@ TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* 
     p.part_ml = p.part_o + (size_t)sms * 2 * qt * BLOCK_M * d;
     p.error_flag = tff_device_error_flag();
     if (p.error_flag == nullptr) return TFF_ERR_LAUNCH;
-    if (d == 128) return qt == 2 ? launch<128, 2>(tm, p, sms, stream) : launch<128, 1>(tm, p, sms, stream);
-    return qt == 2 ? launch<64, 2>(tm, p, sms, stream) : launch<64, 1>(tm, p, sms, stream);
+    if (d == 128) return qt == 2 ? launch<128, 2>(tm, tq, p, sms, stream) : launch<128, 1>(tm, tq, p, sms, stream);
+    return qt == 2 ? launch<64, 2>(tm, tq, p, sms, stream) : launch<64, 1>(tm, tq, p, sms, stream);
 }

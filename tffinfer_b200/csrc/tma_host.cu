@@ -136,6 +136,35 @@ bool tff_tensor_map_kv_groups(const void* cache, long long total_rows, int head_
     return true;
 }
 
+bool tff_tensor_map_heads(const void* q, long long tokens, int kv_heads, int group, int head_dim, int box_tokens, CUtensorMap* out) {
+    static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
+    const MapKey key{q, tokens, head_dim, group, box_tokens, -6, kv_heads};
+    {
+        std::lock_guard<std::mutex> g(g_mu);
+        auto it = cache.find(key);
+        if (it != cache.end()) { *out = it->second; return true; }
+    }
+    EncodeTiledFn enc = get_encode_fn();
+    if (!enc) return false;
+    const cuuint64_t row = (cuuint64_t)head_dim * 2;
+    const cuuint64_t dims[5] = {64, (cuuint64_t)group, (cuuint64_t)head_dim / 64, (cuuint64_t)kv_heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[4] = {row, 128, row * group, row * group * kv_heads};
+    const cuuint32_t box[5] = {64, (cuuint32_t)group, 1, 1, (cuuint32_t)box_tokens};
+    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    CUtensorMap m;
+    if (enc(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(q), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return false;
+    {
+        std::lock_guard<std::mutex> g(g_mu);
+        if (cache.size() > 4096) cache.clear();
+        cache[key] = m;
+    }
+    *out = m;
+    return true;
+}
+
 int* tff_device_error_flag() {
     std::lock_guard<std::mutex> g(g_mu);
     if (g_error_flag) return g_error_flag;

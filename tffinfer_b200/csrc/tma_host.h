@@ -23,6 +23,11 @@ bool tff_tensor_map_kv_page(const void* cache, long long total_rows, int head_di
 bool tff_tensor_map_kv_groups(const void* cache, long long total_rows, int head_dim, int page_size, int kv_heads,
                               CUtensorMap* out);
 
+// Tensor map of bfloat16 rows [tokens, kv_heads * group * head_dim] whose box is 64 columns of the ``group`` query heads of a
+// kv head, of ``box_tokens`` tokens one behind the other (zeros behind the last), with 128-byte swizzle.  Coordinates are
+// (0, 0, 64-column half, kv head, first token).
+bool tff_tensor_map_heads(const void* q, long long tokens, int kv_heads, int group, int head_dim, int box_tokens, CUtensorMap* out);
+
 // Device pointer to the error word (allocated and cleared at first use; nullptr on failure).
 int* tff_device_error_flag();
 
