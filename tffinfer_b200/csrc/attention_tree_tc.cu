@@ -43,7 +43,7 @@ using tc5::tc_fence_after;
 using tc5::tmem_ld16;
 using tc5::tmem_ld_wait;
 
-constexpr int BLOCK_M = 128, BLOCK_N = 64, BARS_PER_TILE = 17, JOIN_ROWS = 32;
+constexpr int BLOCK_M = 128, BLOCK_N = 64, BARS_PER_TILE = 17, JOIN_ROWS = 16;
 constexpr float RESCALE_THRESHOLD = 8.0f;            // in log2 units
 
 struct TreeTcParams {
@@ -330,7 +330,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const __grid_c
             constexpr uint32_t idesc_s = make_idesc(BLOCK_M, BLOCK_N, 0);
             bool ok = true;
             uint32_t phase = 0, phase_q = 0, phase_s = 1;          // of the ring, the queries, s_free (nothing to wait for at first)
-            uint32_t phase_p[2] = {0, 0};
+            uint32_t phase_p = 0;                                  // of p_full, a bit a group
             int st = 0, st_pv = 0;                                 // stages of S(n) and of PV(n - 2)
             while (ok && piece.next(p, rows)) {
                 if (piece.tile * rows + x * p.tile_rows >= piece.w.nodes * G) {
@@ -376,9 +376,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const __grid_c
                     }
                     const int j = n - 2;
                     if (j >= 0) {
-                        ok = mbar_wait_warp(p_full(x, j & 1), phase_p[j & 1], abort_flag);   // P(j) is in tensor memory
+                        ok = mbar_wait_warp(p_full(x, j & 1), phase_p >> (j & 1) & 1u, abort_flag);   // P(j) is in tensor memory
                         if (!ok) break;
-                        phase_p[j & 1] ^= 1;
+                        phase_p ^= 1u << (j & 1);
                         tc_fence_after();
                         const uint64_t vd = vdesc + (uint64_t)(st_pv * (STAGE_BYTES >> 4));
                         umma4_ts<(2 * GROUP >> 4)>(t_o, t_s + 64 + (j & 1) * 32, vd, idesc_pv, j > 0 ? 1u : 0u);
@@ -427,7 +427,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const __grid_c
                 soft_sync();
             }
             const int depth = exists() ? tree_depth(parent, tok) : -1;         // (-1: a row of no node that is there)
-            if (warp == 0) {                                       // the next piece, while the first products run
+            if (warp == 7) {                                       // the next piece, while the first products run (block 1 is this warp's first)
                 Pieces next = now->p;
                 const bool go = next.next(p, rows);
                 Present* to = present + (now == present);
@@ -671,16 +671,17 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const __grid_c
 }
 
 // Joins the pieces of the walks that are more than one share's: a block takes JOIN_ROWS rows of the walk that ends in share
-// blockIdx.x; eight threads a row, each every eighth four of its columns.
+// blockIdx.x; eight threads a row, each an eighth of its columns.  Neighbouring threads have neighbouring rows, whose fours of columns lie
+// side by side (with neighbouring columns instead, at 16 bytes of a line each, the loads came at a quarter of the rate).
 template <int D, int QT>
-__global__ void __launch_bounds__(JOIN_ROWS * 8) attn_tree_join_kernel(const TreeTcParams p) {
-    constexpr int ROWS = QT * BLOCK_M, FOURS = D / 32, AHEAD = 4;
+__global__ void __launch_bounds__(JOIN_ROWS * 8, 8) attn_tree_join_kernel(const TreeTcParams p) {
+    constexpr int ROWS = QT * BLOCK_M, FOURS = D / 32, AHEAD = 2;
     pdl_launch_dependents();
     pdl_wait();
     const int4 join = __ldcg(p.joins + blockIdx.x);                // request, kv head, tile, the first share
     if (join.x < 0) return;
     const int b = join.x, last = blockIdx.x;
-    const int row = blockIdx.y * JOIN_ROWS + threadIdx.x / 8, c = threadIdx.x % 8;
+    const int row = blockIdx.y * JOIN_ROWS + threadIdx.x % JOIN_ROWS, c = threadIdx.x / JOIN_ROWS * FOURS;
     const int R = (join.z * QT + row / BLOCK_M) * p.tile_rows + row % BLOCK_M;
     const int q0 = p.q_start[b], rows_total = min(p.q_start[b + 1] - q0, TREE_MAX_NODES) * p.group;
     if (row % BLOCK_M >= p.tile_rows || R >= rows_total) return;
@@ -697,7 +698,7 @@ __global__ void __launch_bounds__(JOIN_ROWS * 8) attn_tree_join_kernel(const Tre
             const size_t slot = (size_t)s * 2 + (s == join.w ? 1 : 0);
             ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + slot * ROWS + row);
 #pragma unroll
-            for (int k = 0; k < FOURS; ++k) v[i][k] = __ldcg(reinterpret_cast<const float4*>(p.part_o) + (slot * (D / 4) + k * 8 + c) * ROWS + row);
+            for (int k = 0; k < FOURS; ++k) v[i][k] = __ldcg(reinterpret_cast<const float4*>(p.part_o) + (slot * (D / 4) + c + k) * ROWS + row);
         }
         // (a piece that the row saw nothing of counts for nothing)
         float most = m;
@@ -723,13 +724,14 @@ __global__ void __launch_bounds__(JOIN_ROWS * 8) attn_tree_join_kernel(const Tre
     const int tok = node_of(p, R), t = q0 + tok, h = join.y * p.group + (R - tok * p.group);
     float inv = 0.f;
     if (l > 0.f) inv = (p.gate ? __ldcg(p.gate + (size_t)t * p.nq + h) : 1.f) / (p.sink ? l + exp2f(attn_sink_log2(p.sink_val, h) - m) : l);
+    uint4* to = reinterpret_cast<uint4*>(p.out + ((size_t)t * p.nq + h) * D + c * 4);
+    auto pair = [&](float a, float b2) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a * inv, b2 * inv);
+        return l > 0.f ? *reinterpret_cast<const uint32_t*>(&v) : 0u;
+    };
 #pragma unroll
-    for (int k = 0; k < FOURS; ++k) {
-        __nv_bfloat162 lo = __floats2bfloat162_rn(o[k].x * inv, o[k].y * inv), hi = __floats2bfloat162_rn(o[k].z * inv, o[k].w * inv);
-        if (!(l > 0.f)) lo = hi = __floats2bfloat162_rn(0.f, 0.f);
-        *reinterpret_cast<uint2*>(p.out + ((size_t)t * p.nq + h) * D + (k * 8 + c) * 4) =
-            make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
-    }
+    for (int k = 0; k < FOURS; k += 2)
+        to[k / 2] = make_uint4(pair(o[k].x, o[k].y), pair(o[k].z, o[k].w), pair(o[k + 1].x, o[k + 1].y), pair(o[k + 1].z, o[k + 1].w));
 }
 
 template <int D, int QT>
