@@ -674,8 +674,8 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const __grid_c
 // blockIdx.x; eight threads a row, each an eighth of its columns.  Neighbouring threads have neighbouring rows, whose fours of columns lie
 // side by side (with neighbouring columns instead, at 16 bytes of a line each, the loads came at a quarter of the rate).
 template <int D, int QT>
-__global__ void __launch_bounds__(JOIN_ROWS * 8, 8) attn_tree_join_kernel(const TreeTcParams p) {
-    constexpr int ROWS = QT * BLOCK_M, FOURS = D / 32, AHEAD = 2;
+__global__ void __launch_bounds__(JOIN_ROWS * 8) attn_tree_join_kernel(const TreeTcParams p) {
+    constexpr int ROWS = QT * BLOCK_M, FOURS = D / 32, AHEAD = 4;
     pdl_launch_dependents();
     pdl_wait();
     const int4 join = __ldcg(p.joins + blockIdx.x);                // request, kv head, tile, the first share
@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(JOIN_ROWS * 8, 8) attn_tree_join_kernel(const 
 }
 
 template <int D, int QT>
-int launch(const CUtensorMap& tm, const CUtensorMap& tq, const TreeTcParams& p, int ctas, cudaStream_t stream) {
+int launch(const CUtensorMap& tm, const CUtensorMap& tq, const TreeTcParams& p, int ctas, int rows, cudaStream_t stream) {
     constexpr int smem = TreeCfg<D, QT>::kSmem;
     auto kern = attn_tree_tc_kernel<D, QT>;
     static bool configured = false;
@@ -745,7 +745,7 @@ int launch(const CUtensorMap& tm, const CUtensorMap& tq, const TreeTcParams& p, 
     }
     const int st = tff_launch_pdl(kern, dim3(ctas), dim3(TreeCfg<D, QT>::kThreads), (size_t)smem, stream, tm, tq, p);
     if (st != TFF_OK || p.whole) return st;
-    return tff_launch_pdl(attn_tree_join_kernel<D, QT>, dim3(ctas, QT * BLOCK_M / JOIN_ROWS), dim3(JOIN_ROWS * 8), (size_t)0, stream, p);
+    return tff_launch_pdl(attn_tree_join_kernel<D, QT>, dim3(ctas, (rows + JOIN_ROWS - 1) / JOIN_ROWS), dim3(JOIN_ROWS * 8), (size_t)0, stream, p);
 }
 
 }  // namespace
@@ -795,6 +795,6 @@ TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* 
     p.part_ml = p.part_o + (size_t)sms * 2 * qt * BLOCK_M * d;
     p.error_flag = tff_device_error_flag();
     if (p.error_flag == nullptr) return TFF_ERR_LAUNCH;
-    if (d == 128) return qt == 2 ? launch<128, 2>(tm, tq, p, sms, stream) : launch<128, 1>(tm, tq, p, sms, stream);
-    return qt == 2 ? launch<64, 2>(tm, tq, p, sms, stream) : launch<64, 1>(tm, tq, p, sms, stream);
+    if (d == 128) return qt == 2 ? launch<128, 2>(tm, tq, p, sms, qt == 2 ? 2 * BLOCK_M : max_nodes * group, stream) : launch<128, 1>(tm, tq, p, sms, qt == 2 ? 2 * BLOCK_M : max_nodes * group, stream);
+    return qt == 2 ? launch<64, 2>(tm, tq, p, sms, qt == 2 ? 2 * BLOCK_M : max_nodes * group, stream) : launch<64, 1>(tm, tq, p, sms, qt == 2 ? 2 * BLOCK_M : max_nodes * group, stream);
 }

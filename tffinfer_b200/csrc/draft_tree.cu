@@ -52,6 +52,8 @@ accept_tree_kernel(const int* tokens, const int* parents, const int* drawn, cons
     if (lane == 0) count[b] = k;
 }
 
+constexpr int KEEP_THREADS = 256, AHEAD = 8;
+
 struct KeepParams {
     char* cache; long long page_bytes, layer_bytes, plane_bytes, head_bytes;
     int pages, layers, planes, heads, page_size, row_bytes;
@@ -60,40 +62,44 @@ struct KeepParams {
 };
 
 // Slot pos + path[j] -> slot pos + j, for j < count, in every layer, plane and head.  A thread takes one V of a row for all j in
-// order, four loads ahead of their stores: a path's nodes ascend, so what is stored at j is never read at a later j.
+// order, eight loads ahead of their stores: a path's nodes ascend, so what is stored at j is never read at a later j.  The slots'
+// places in a (layer, plane, head) are worked out once a block.
 template <typename V>
-__global__ void __launch_bounds__(256) keep_path_kernel(const KeepParams p) {
+__global__ void __launch_bounds__(KEEP_THREADS) keep_path_kernel(const KeepParams p) {
+    __shared__ long long from[AHEAD], to[AHEAD];     // -1: nothing to move
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.y;
     const int n = min(__ldcg(p.count + b), p.width);
+    if (n <= 1) return;
     const int row = p.row_bytes / (int)sizeof(V);
-    const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (n <= 1 || item >= (long long)p.layers * p.planes * p.heads * row) return;
+    const long long item = (long long)blockIdx.x * KEEP_THREADS + threadIdx.x;
+    const bool mine = item < (long long)p.layers * p.planes * p.heads * row;
     const int c = (int)(item % row), h = (int)(item / row % p.heads), q = (int)(item / row / p.heads % p.planes);
     const int layer = (int)(item / row / p.heads / p.planes);
     char* base = p.cache + layer * p.layer_bytes + q * p.plane_bytes + h * p.head_bytes + c * (int)sizeof(V);
     const int pos = p.pos_start[b];
-    const int* table = p.block_table + (size_t)b * p.table_width;
-    auto slot = [&](int i) -> V* {
-        const long long at = (long long)pos + i;
-        if (i < 0 || at < 0 || at / p.page_size >= p.table_width) return nullptr;
-        const int page = table[at / p.page_size];
-        if (page < 0 || page >= p.pages) return nullptr;
-        return (V*)(base + page * p.page_bytes + at % p.page_size * p.row_bytes);
-    };
-    for (int j0 = 1; j0 < n; j0 += 4) {
-        V v[4];
-        V *from[4], *to[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int j = j0 + u, i = j < n ? __ldcg(p.path + (size_t)b * p.width + j) : j;
-            from[u] = i != j ? slot(i) : nullptr;
-            to[u] = from[u] ? slot(j) : nullptr;
-            if (to[u]) v[u] = __ldcg(from[u]);
+    for (int j0 = 1; j0 < n; j0 += AHEAD) {
+        if (j0 > 1) __syncthreads();                 // (the slots before have been read)
+        if (threadIdx.x < 2 * AHEAD) {
+            const int j = j0 + threadIdx.x % AHEAD, i = j < n ? __ldcg(p.path + (size_t)b * p.width + j) : j;
+            const long long at = (long long)pos + (threadIdx.x < AHEAD ? i : j);
+            long long place = -1;
+            if (i != j && i >= 0 && at >= 0 && at / p.page_size < p.table_width) {
+                const int page = p.block_table[(size_t)b * p.table_width + at / p.page_size];
+                if (page >= 0 && page < p.pages) place = page * p.page_bytes + at % p.page_size * p.row_bytes;
+            }
+            (threadIdx.x < AHEAD ? from : to)[threadIdx.x % AHEAD] = place;
         }
+        __syncthreads();
+        if (!mine) continue;
+        V v[AHEAD];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) if (to[u]) *to[u] = v[u];
+        for (int u = 0; u < AHEAD; ++u)
+            if (from[u] >= 0 && to[u] >= 0) v[u] = __ldcg((const V*)(base + from[u]));
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (from[u] >= 0 && to[u] >= 0) *(V*)(base + to[u]) = v[u];
     }
 }
 
@@ -125,10 +131,10 @@ TFF_API int tff_keep_path(void* cache, int pages, int layers, int planes, int he
     const unsigned long long align = (uintptr_t)cache | (unsigned long long)page_bytes | (unsigned long long)layer_bytes | (unsigned long long)row_bytes;
     const int v = align % 16 == 0 ? 16 : align % 4 == 0 ? 4 : 2;
     const long long items = (long long)layers * planes * heads * (row_bytes / v);
-    const long long blocks = (items + 255) / 256;
+    const long long blocks = (items + KEEP_THREADS - 1) / KEEP_THREADS;
     if (blocks > 0x7fffffff) return TFF_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)blocks, requests);
-    if (v == 16) return tff_launch_pdl(keep_path_kernel<uint4>, grid, dim3(256), (size_t)0, stream, p);
-    if (v == 4) return tff_launch_pdl(keep_path_kernel<unsigned>, grid, dim3(256), (size_t)0, stream, p);
-    return tff_launch_pdl(keep_path_kernel<unsigned short>, grid, dim3(256), (size_t)0, stream, p);
+    if (v == 16) return tff_launch_pdl(keep_path_kernel<uint4>, grid, dim3(KEEP_THREADS), (size_t)0, stream, p);
+    if (v == 4) return tff_launch_pdl(keep_path_kernel<unsigned>, grid, dim3(KEEP_THREADS), (size_t)0, stream, p);
+    return tff_launch_pdl(keep_path_kernel<unsigned short>, grid, dim3(KEEP_THREADS), (size_t)0, stream, p);
 }

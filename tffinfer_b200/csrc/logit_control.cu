@@ -10,15 +10,18 @@
 // The logits are read once and written once; what is added to that traffic is the history, and a bit a token of a mask.
 //
 // A CTA takes a slice of the vocabulary for all rows of one request: it counts the history's tokens of its slice in shared
-// memory (integers: in any order), once for all rows, and then streams the rows' slices.  The few tokens of a row's
-// path and the few biased ones are put right behind that pass, by the same CTA.
+// memory (integers: in any order), once for all rows, and then streams the rows' slices, four logits a load and four loads a
+// thread on their way.  The few tokens of a row's path and the few biased ones are put right behind that pass, by the
+// same CTA.  Where a mask allows none of a load's four tokens nothing is read.
 #include "common.cuh"
+#include "tma_host.h"
 
 namespace {
 
-constexpr int NT = 256;
+constexpr int NT = 256, CTAS_AN_SM = 4;
 constexpr int MAX_NODES = 256;                       // of a request's tree
-constexpr unsigned PROMPT = 0x80000000u;             // a count's top bit: seen in the prompt
+constexpr int ROWS_AT_ONCE = 256;
+constexpr int MOST_TOKENS = 20480, LEAST_TOKENS = 1024;        // of a slice: 40 KB of counts leave room for four CTAs an SM
 
 struct ControlParams {
     const float* logits; float* out;
@@ -30,95 +33,209 @@ struct ControlParams {
     const int *parents, *tokens;
 };
 
+// The tokens of a slice as counts: 16 bits a token while no count can pass 32,767, else 32 bits, of half as many tokens.  The top
+// bit: seen in the prompt.
+struct Counts {
+    unsigned* words;
+    bool wide;
+    __device__ __forceinline__ void prompt(int i) {
+        if (wide) atomicOr(words + i, 0x80000000u);
+        else atomicOr(words + (i >> 1), 0x8000u << (i & 1) * 16);
+    }
+    __device__ __forceinline__ void add(int i) {
+        if (wide) atomicAdd(words + i, 1u);
+        else atomicAdd(words + (i >> 1), 1u << (i & 1) * 16);
+    }
+    // (a count's top bit as the top bit of 32)
+    __device__ __forceinline__ unsigned at(int i) const {
+        if (wide) return words[i];
+        const unsigned c = reinterpret_cast<const unsigned short*>(words)[i];
+        return (c & 0x8000u) << 16 | (c & 0x7fffu);
+    }
+};
+
 __device__ __forceinline__ float penalised(float x, unsigned count, unsigned more, float rep, float freq, float pres) {
-    const unsigned n = (count & ~PROMPT) + more;
+    const unsigned n = (count & 0x7fffffffu) + more;
     if (count | more) x = x > 0.f ? x / rep : x * rep;
     return n ? x - (freq * (float)n + pres) : x;
 }
 
-__global__ void __launch_bounds__(NT) control_kernel(const ControlParams p) {
-    extern __shared__ unsigned counts[];             // [slice]
+// VEC: logits and outputs lie alike within 16 bytes.
+template <bool VEC>
+__global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlParams p) {
+    extern __shared__ unsigned count_words[];        // [slice / 2]
+    __shared__ int mask_at[ROWS_AT_ONCE];
     __shared__ short parent[MAX_NODES];
     __shared__ int token[MAX_NODES];
+    __shared__ int bias_range[2];                    // of the slice
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.y, lo = blockIdx.x * p.slice, hi = min(p.vocab, lo + p.slice);
+    const int b = blockIdx.y;
     const int r0 = max(0, p.row_start[b]), r1 = min(p.rows, p.row_start[b + 1]);
     if (r0 >= r1) return;
     const float rep = p.settings[3 * b], freq = p.settings[3 * b + 1], pres = p.settings[3 * b + 2];
     const bool counted = rep != 1.f || freq != 0.f || pres != 0.f;
-    const int nodes = p.parents ? min(r1 - r0, MAX_NODES) : 0;
-    for (int i = threadIdx.x; i < hi - lo; i += NT) counts[i] = 0u;
+    const long long first_token = p.history_start[b];
+    const int len = first_token < 0 ? 0 : (int)max(0ll, min((long long)p.history_len[b], p.history_size - first_token));
+    const int prompt = p.prompt_len[b];
+    Counts counts;
+    counts.words = count_words;
+    counts.wide = len > 32767;
+    const int e0 = p.bias_start ? max(0, p.bias_start[b]) : 0, e1 = p.bias_start ? min(p.biases, p.bias_start[b + 1]) : 0;
+    const bool biased = e0 < e1;
+    const int nodes = p.parents && counted ? min(r1 - r0, MAX_NODES) : 0;
     for (int i = threadIdx.x; i < nodes; i += NT) {
         const int up = __ldcg(p.parents + r0 + i);
         parent[i] = (short)(up < -1 || up >= i ? -2 : up);
         token[i] = __ldcg(p.tokens + r0 + i);
     }
-    __syncthreads();
-    if (counted) {
-        const long long first = p.history_start[b];
-        const long long len = first < 0 ? 0 : min((long long)p.history_len[b], p.history_size - first);
-        const int prompt = p.prompt_len[b];
-        for (int i = threadIdx.x; i < len; i += NT) {
-            const int t = __ldcg(p.history + first + i);
-            if (t >= lo && t < hi) {
-                if (i < prompt) atomicOr(&counts[t - lo], PROMPT);
-                else atomicAdd(&counts[t - lo], 1u);
-            }
-        }
-        __syncthreads();
-    }
-    auto mask_of = [&](int r) -> const unsigned* {
+    auto allowed = [&](int m, int t) { return m < 0 || (__ldcg(p.mask + (size_t)m * p.mask_words + (t >> 5)) >> (t & 31) & 1u); };
+    auto mask_of = [&](int r) {
         const int m = p.mask ? (p.mask_row ? __ldcg(p.mask_row + r) : r) : -1;
-        return m >= 0 && m < p.mask_rows ? p.mask + (size_t)m * p.mask_words : nullptr;
+        return m < p.mask_rows ? m : -1;
     };
-    auto allowed = [&](const unsigned* mask, int t) { return mask == nullptr || (__ldcg(mask + (t >> 5)) >> (t & 31) & 1u); };
-    for (int r = r0; r < r1; ++r) {
-        const float* in = p.logits + (size_t)r * p.vocab;
-        float* to = p.out + (size_t)r * p.vocab;
-        const unsigned* mask = mask_of(r);
-        for (int t = lo + threadIdx.x; t < hi; t += NT) {
-            const float x = penalised(__ldcg(in + t), counts[t - lo], 0u, rep, freq, pres);
-            to[t] = allowed(mask, t) ? x : -INFINITY;
-        }
-    }
-    if (nodes > 0 && counted) {
-        __syncthreads();
-        // the tokens of a node's path, a thread a node; one that is there more than once is done where the path has it first
-        for (int i = threadIdx.x; i < nodes; i += NT) {
-            int root = i;
-            while (root >= 0) root = parent[root];
-            if (root != -1) continue;                // padding, or a node behind it: no path
-            const float* in = p.logits + (size_t)(r0 + i) * p.vocab;
-            float* to = p.out + (size_t)(r0 + i) * p.vocab;
-            const unsigned* mask = mask_of(r0 + i);
-            for (int a = i; a >= 0; a = parent[a]) {
-                const int t = token[a];
-                if (t < lo || t >= hi) continue;
-                unsigned more = 1;
-                bool first = true;
-                for (int o = i; o > a; o = parent[o]) first = first && token[o] != t;
-                for (int o = parent[a]; o >= 0; o = parent[o]) more += token[o] == t;
-                if (!first) continue;
-                const float x = penalised(__ldcg(in + t), counts[t - lo], more, rep, freq, pres);
-                to[t] = allowed(mask, t) ? x : -INFINITY;
+    const int end = min(p.vocab, (int)(blockIdx.x + 1) * p.slice), width = counts.wide ? p.slice / 2 : p.slice;
+    for (int lo = blockIdx.x * p.slice; lo < end; lo += width) {
+        const int hi = min(end, lo + width);
+        __syncthreads();                             // (the part before is through with the counts)
+        if (counted) {
+            for (int i = threadIdx.x; i < p.slice / 2; i += NT) count_words[i] = 0u;
+            __syncthreads();
+            for (int i0 = threadIdx.x; i0 < len; i0 += 8 * NT) {
+                int t[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) t[u] = i0 + u * NT < len ? __ldcg(p.history + first_token + i0 + u * NT) : -1;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    if (t[u] < lo || t[u] >= hi) continue;
+                    if (i0 + u * NT < prompt) counts.prompt(t[u] - lo);
+                    else counts.add(t[u] - lo);
+                }
             }
         }
-    }
-    if (p.bias_start) {
-        __syncthreads();
-        // ascending tokens: equal ones are neighbours, whose values the first of them adds in their order
-        const int e0 = max(0, p.bias_start[b]), e1 = min(p.biases, p.bias_start[b + 1]);
-        for (int e = e0 + threadIdx.x; e < e1; e += NT) {
-            const int t = p.bias_tokens[e];
-            if (t < lo || t >= hi || (e > e0 && p.bias_tokens[e - 1] == t)) continue;
-            float bias = p.bias_values[e];
-            for (int o = e + 1; o < e1 && p.bias_tokens[o] == t; ++o) bias += p.bias_values[o];
-            for (int r = r0; r < r1; ++r) {
+        for (int c0 = r0; c0 < r1; c0 += ROWS_AT_ONCE) {
+            const int rows = min(ROWS_AT_ONCE, r1 - c0);
+            if (c0 > r0) __syncthreads();
+            for (int i = threadIdx.x; i < rows; i += NT) mask_at[i] = mask_of(c0 + i);
+            __syncthreads();
+            auto one = [&](int row, int t) {
+                const size_t at = (size_t)(c0 + row) * p.vocab + t;
+                const float x = __ldcg(p.logits + at);
+                p.out[at] = allowed(mask_at[row], t) ? penalised(x, counted ? counts.at(t - lo) : 0u, 0u, rep, freq, pres) : -INFINITY;
+            };
+            if (!VEC) {
+                for (int row = 0; row < rows; ++row)
+                    for (int t = lo + threadIdx.x; t < hi; t += NT) one(row, t);
+                continue;
+            }
+            // tokens ahead of a row's first aligned four
+            auto skip = [&](int row) {
+                return (int)((4 - (((uintptr_t)p.logits >> 2) + (size_t)(c0 + row) * p.vocab + lo)) & 3);
+            };
+            const int fours = (hi - lo + 3) / 4;
+            for (int i0 = threadIdx.x; i0 < rows * fours; i0 += 4 * NT) {
+                float4 x[4];
+                unsigned bits[4];
+                int row[4], t[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int i = i0 + u * NT;
+                    row[u] = i / fours;
+                    t[u] = row[u] < rows ? lo + skip(row[u]) + (i - row[u] * fours) * 4 : hi;
+                    bits[u] = t[u] + 4 <= hi ? 15u : 0u;
+                    const int m = bits[u] ? mask_at[row[u]] : -1;
+                    if (m >= 0) {
+                        const unsigned* w = p.mask + (size_t)m * p.mask_words + (t[u] >> 5);
+                        const unsigned low = __ldcg(w), high = (t[u] & 31) > 28 ? __ldcg(w + 1) : 0u;
+                        bits[u] = __funnelshift_r(low, high, t[u] & 31) & 15u;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (bits[u]) x[u] = __ldcg(reinterpret_cast<const float4*>(p.logits + (size_t)(c0 + row[u]) * p.vocab + t[u]));
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (t[u] + 4 > hi) continue;
+                    if (counted) {
+                        const int at = t[u] - lo;
+                        x[u].x = penalised(x[u].x, counts.at(at), 0u, rep, freq, pres);
+                        x[u].y = penalised(x[u].y, counts.at(at + 1), 0u, rep, freq, pres);
+                        x[u].z = penalised(x[u].z, counts.at(at + 2), 0u, rep, freq, pres);
+                        x[u].w = penalised(x[u].w, counts.at(at + 3), 0u, rep, freq, pres);
+                    }
+                    if (!(bits[u] & 1u)) x[u].x = -INFINITY;
+                    if (!(bits[u] & 2u)) x[u].y = -INFINITY;
+                    if (!(bits[u] & 4u)) x[u].z = -INFINITY;
+                    if (!(bits[u] & 8u)) x[u].w = -INFINITY;
+                    *reinterpret_cast<float4*>(p.out + (size_t)(c0 + row[u]) * p.vocab + t[u]) = x[u];
+                }
+            }
+            // the up to three tokens of a row ahead of its fours, and those behind
+            for (int i = threadIdx.x; i < rows * 6; i += NT) {
+                const int row = i / 6, e = i % 6, s = skip(row), left = (hi - lo - s) & 3;
+                if (hi - lo < s) {                   // (a slice of fewer tokens than that)
+                    if (e < hi - lo) one(row, lo + e);
+                } else if (e < 3 ? e < s : e - 3 < left) {
+                    one(row, e < 3 ? lo + e : hi - left + e - 3);
+                }
+            }
+        }
+        if (nodes > 0) {
+            __syncthreads();
+            // the tokens of a node's path, a thread a node; one that is there more than once is done where the path has it first
+            for (int i = threadIdx.x; i < nodes; i += NT) {
+                int root = i;
+                while (root >= 0) root = parent[root];
+                if (root != -1) continue;            // padding, or a node behind it: no path
+                const size_t at = (size_t)(r0 + i) * p.vocab;
+                const int m = mask_of(r0 + i);
+                for (int a = i; a >= 0; a = parent[a]) {
+                    const int t = token[a];
+                    if (t < lo || t >= hi) continue;
+                    unsigned more = 1;
+                    bool first = true;
+                    for (int o = i; o > a; o = parent[o]) first = first && token[o] != t;
+                    for (int o = parent[a]; o >= 0; o = parent[o]) more += token[o] == t;
+                    if (!first) continue;
+                    const float x = penalised(__ldcg(p.logits + at + t), counts.at(t - lo), more, rep, freq, pres);
+                    p.out[at + t] = allowed(m, t) ? x : -INFINITY;
+                }
+            }
+        }
+        if (biased) {
+            if (threadIdx.x == 0) { bias_range[0] = e1; bias_range[1] = e0; }
+            __syncthreads();
+            for (int e = e0 + threadIdx.x; e < e1; e += NT) {
+                const int t = p.bias_tokens[e];
+                if (t >= lo && t < hi) { atomicMin(&bias_range[0], e); atomicMax(&bias_range[1], e + 1); }
+            }
+            __syncthreads();
+            // ascending tokens: equal ones are neighbours, whose values the first of them adds in their order
+            const int f0 = bias_range[0], f1 = bias_range[1], n = r1 - r0;
+            for (long long i = threadIdx.x; i < (long long)(f1 - f0) * n; i += NT) {
+                const int e = f0 + (int)(i / n), r = r0 + (int)(i % n);
+                const int t = p.bias_tokens[e];
+                if (t < lo || t >= hi || (e > e0 && p.bias_tokens[e - 1] == t)) continue;
+                float bias = p.bias_values[e];
+                for (int o = e + 1; o < e1 && p.bias_tokens[o] == t; ++o) bias += p.bias_values[o];
                 float* to = p.out + (size_t)r * p.vocab + t;
                 *to = bias == -INFINITY ? bias : *to + bias;
             }
         }
+    }
+}
+
+// Tokens of a slice: as many slices a request as fill whole waves of four CTAs an SM, of few tokens where there are few
+// requests.
+int slice_tokens(int vocab, int requests, int sms) {
+    const long long slots = (long long)CTAS_AN_SM * (sms > 0 ? sms : 1);
+    for (int wave = 1;; ++wave) {
+        const long long slices = wave * slots / requests;
+        if (slices < 1) continue;
+        const long long tokens = ((vocab + slices - 1) / slices + 7) / 8 * 8;
+        if (tokens <= MOST_TOKENS) return (int)(tokens < LEAST_TOKENS ? LEAST_TOKENS : tokens);
     }
 }
 
@@ -142,6 +259,9 @@ TFF_API int tff_control_logits(const float* logits, float* out, int rows, int vo
     p.bias_start = bias_start; p.bias_tokens = bias_tokens; p.bias_values = bias_values; p.biases = biases;
     p.mask = (const unsigned*)mask; p.mask_rows = mask_rows; p.mask_words = mask_words; p.mask_row = mask_row;
     p.parents = parents; p.tokens = tokens;
-    p.slice = 4096;
-    return tff_launch_pdl(control_kernel, dim3((vocab + p.slice - 1) / p.slice, requests), dim3(NT), (size_t)p.slice * 4, stream, p);
+    p.slice = slice_tokens(vocab, requests, tff_num_sms());
+    const dim3 grid((vocab + p.slice - 1) / p.slice, requests);
+    const size_t smem = (size_t)p.slice * 2;
+    if ((((uintptr_t)logits ^ (uintptr_t)out) & 15) == 0) return tff_launch_pdl(control_kernel<true>, grid, dim3(NT), smem, stream, p);
+    return tff_launch_pdl(control_kernel<false>, grid, dim3(NT), smem, stream, p);
 }
