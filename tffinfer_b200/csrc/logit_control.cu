@@ -11,7 +11,7 @@
 //
 // A CTA takes a slice of the vocabulary for all rows of one request: it counts the history's tokens of its slice in shared
 // memory (integers: in any order), once for all rows, and then streams the rows' slices, four logits a load and four loads a
-// thread on their way.  The few tokens of a row's path and the few biased ones are put right behind that pass, by the
+// thread on their way, of four rows where there are as many.  The few tokens of a row's path and the few biased ones are put right behind that pass, by the
 // same CTA.  Where a mask allows none of a load's four tokens nothing is read.
 #include "common.cuh"
 #include "tma_host.h"
@@ -21,7 +21,8 @@ namespace {
 constexpr int NT = 256, CTAS_AN_SM = 4;
 constexpr int MAX_NODES = 256;                       // of a request's tree
 constexpr int ROWS_AT_ONCE = 256;
-constexpr int MOST_TOKENS = 20480, LEAST_TOKENS = 1024;        // of a slice: 40 KB of counts leave room for four CTAs an SM
+constexpr int MOST_TOKENS = 16384, LEAST_TOKENS = 1024;        // of a slice: 32 KB of counts leave room for four CTAs an SM
+constexpr int MASK_WORDS = 2048;                     // of masks in shared memory: a part of the rows' at a time
 
 struct ControlParams {
     const float* logits; float* out;
@@ -54,17 +55,26 @@ struct Counts {
     }
 };
 
-__device__ __forceinline__ float penalised(float x, unsigned count, unsigned more, float rep, float freq, float pres) {
-    const unsigned n = (count & 0x7fffffffu) + more;
-    if (count | more) x = x > 0.f ? x / rep : x * rep;
-    return n ? x - (freq * (float)n + pres) : x;
-}
+// A request's penalties.  A positive logit is multiplied by 1 / repetition, rounded once for the request: a second rounding in
+// float32 (2^-24) in place of a division, which with its branches took most of the kernel's instructions.
+struct Penalties {
+    float rep, inverse, freq, pres;
+    // ``count`` as Counts gives it; ``more`` times on the row's path.  What was not seen keeps its bits.
+    __device__ __forceinline__ float operator()(float x, unsigned count, unsigned more = 0u) const {
+        const unsigned n = (count & 0x7fffffffu) + more;
+        const float factor = (count | more) == 0u ? 1.f : x > 0.f ? inverse : rep;
+        return x * factor - (n ? fmaf(freq, (float)n, pres) : 0.f);
+    }
+};
 
 // VEC: logits and outputs lie alike within 16 bytes.
 template <bool VEC>
 __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlParams p) {
     extern __shared__ unsigned count_words[];        // [slice / 2]
     __shared__ int mask_at[ROWS_AT_ONCE];
+    __shared__ unsigned masks[MASK_WORDS];           // of a part of the rows: [row][words of the slice]
+    __shared__ short hits[MAX_NODES];                // nodes whose tokens lie in the slice
+    __shared__ int hit_count;
     __shared__ short parent[MAX_NODES];
     __shared__ int token[MAX_NODES];
     __shared__ int bias_range[2];                    // of the slice
@@ -73,8 +83,10 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
     const int b = blockIdx.y;
     const int r0 = max(0, p.row_start[b]), r1 = min(p.rows, p.row_start[b + 1]);
     if (r0 >= r1) return;
-    const float rep = p.settings[3 * b], freq = p.settings[3 * b + 1], pres = p.settings[3 * b + 2];
-    const bool counted = rep != 1.f || freq != 0.f || pres != 0.f;
+    Penalties penalised;
+    penalised.rep = p.settings[3 * b]; penalised.freq = p.settings[3 * b + 1]; penalised.pres = p.settings[3 * b + 2];
+    penalised.inverse = 1.f / penalised.rep;
+    const bool counted = penalised.rep != 1.f || penalised.freq != 0.f || penalised.pres != 0.f;
     const long long first_token = p.history_start[b];
     const int len = first_token < 0 ? 0 : (int)max(0ll, min((long long)p.history_len[b], p.history_size - first_token));
     const int prompt = p.prompt_len[b];
@@ -113,63 +125,118 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
                 }
             }
         }
-        for (int c0 = r0; c0 < r1; c0 += ROWS_AT_ONCE) {
-            const int rows = min(ROWS_AT_ONCE, r1 - c0);
+        // the biases of the slice: a run of the request's
+        if (threadIdx.x == 0) { bias_range[0] = e1; bias_range[1] = e0; hit_count = 0; }
+        __syncthreads();
+        for (int e = e0 + threadIdx.x; e < e1; e += NT) {
+            const int t = p.bias_tokens[e];
+            if (t >= lo && t < hi) { atomicMin(&bias_range[0], e); atomicMax(&bias_range[1], e + 1); }
+        }
+        for (int i = threadIdx.x; i < nodes; i += NT)
+            if (token[i] >= lo && token[i] < hi) hits[atomicAdd(&hit_count, 1)] = (short)i;
+        const int w0 = lo >> 5, words = ((hi - 1) >> 5) - w0 + 1;
+        const int at_once = p.mask ? min(ROWS_AT_ONCE, MASK_WORDS / words) : ROWS_AT_ONCE;
+        for (int c0 = r0; c0 < r1; c0 += at_once) {
+            const int rows = min(at_once, r1 - c0);
             if (c0 > r0) __syncthreads();
             for (int i = threadIdx.x; i < rows; i += NT) mask_at[i] = mask_of(c0 + i);
             __syncthreads();
+            if (p.mask) {
+                for (int i = threadIdx.x; i < rows * words; i += NT) {
+                    const int m = mask_at[i / words];
+                    masks[i] = m < 0 ? 0xffffffffu : __ldcg(p.mask + (size_t)m * p.mask_words + w0 + i % words);
+                }
+                __syncthreads();
+            }
+            auto allowed_here = [&](int row, int t) { return !p.mask || (masks[row * words + (t >> 5) - w0] >> (t & 31) & 1u); };
             auto one = [&](int row, int t) {
                 const size_t at = (size_t)(c0 + row) * p.vocab + t;
                 const float x = __ldcg(p.logits + at);
-                p.out[at] = allowed(mask_at[row], t) ? penalised(x, counted ? counts.at(t - lo) : 0u, 0u, rep, freq, pres) : -INFINITY;
+                p.out[at] = allowed_here(row, t) ? penalised(x, counted ? counts.at(t - lo) : 0u) : -INFINITY;
             };
             if (!VEC) {
                 for (int row = 0; row < rows; ++row)
                     for (int t = lo + threadIdx.x; t < hi; t += NT) one(row, t);
                 continue;
             }
-            // tokens ahead of a row's first aligned four
+            // tokens ahead of a row's first aligned four: the same for every fourth row, and for all where vocab is a multiple of 4
             auto skip = [&](int row) {
                 return (int)((4 - (((uintptr_t)p.logits >> 2) + (size_t)(c0 + row) * p.vocab + lo)) & 3);
             };
-            const int fours = (hi - lo + 3) / 4;
-            for (int i0 = threadIdx.x; i0 < rows * fours; i0 += 4 * NT) {
-                float4 x[4];
-                unsigned bits[4];
-                int row[4], t[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int i = i0 + u * NT;
-                    row[u] = i / fours;
-                    t[u] = row[u] < rows ? lo + skip(row[u]) + (i - row[u] * fours) * 4 : hi;
-                    bits[u] = t[u] + 4 <= hi ? 15u : 0u;
-                    const int m = bits[u] ? mask_at[row[u]] : -1;
-                    if (m >= 0) {
-                        const unsigned* w = p.mask + (size_t)m * p.mask_words + (t[u] >> 5);
-                        const unsigned low = __ldcg(w), high = (t[u] & 31) > 28 ? __ldcg(w + 1) : 0u;
-                        bits[u] = __funnelshift_r(low, high, t[u] & 31) & 15u;
+            const int step = p.vocab & 3 ? 4 : 1;
+            for (int like = 0; like < min(step, rows); ++like) {
+                const int s0 = lo + skip(like), fours = (hi - s0) / 4, alike = (rows - like + step - 1) / step;
+                auto from = [&](int n) { return p.logits + (size_t)(c0 + like + n * step) * p.vocab; };
+                auto bits_of = [&](int n, int t) -> unsigned {
+                    if (!p.mask) return 15u;
+                    const unsigned* w = masks + (like + n * step) * words + (t >> 5) - w0;
+                    const unsigned low = w[0], high = (t & 31) > 28 ? w[1] : 0u;
+                    return __funnelshift_r(low, high, t & 31) & 15u;
+                };
+                auto finish = [&](float4 x, unsigned bits, int n, int t, const unsigned (&c)[4], bool any) {
+                    if (any) {
+                        x.x = penalised(x.x, c[0]);
+                        x.y = penalised(x.y, c[1]);
+                        x.z = penalised(x.z, c[2]);
+                        x.w = penalised(x.w, c[3]);
                     }
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (bits[u]) x[u] = __ldcg(reinterpret_cast<const float4*>(p.logits + (size_t)(c0 + row[u]) * p.vocab + t[u]));
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if (t[u] + 4 > hi) continue;
-                    if (counted) {
-                        const int at = t[u] - lo;
-                        x[u].x = penalised(x[u].x, counts.at(at), 0u, rep, freq, pres);
-                        x[u].y = penalised(x[u].y, counts.at(at + 1), 0u, rep, freq, pres);
-                        x[u].z = penalised(x[u].z, counts.at(at + 2), 0u, rep, freq, pres);
-                        x[u].w = penalised(x[u].w, counts.at(at + 3), 0u, rep, freq, pres);
+                    if (bits != 15u) {
+                        if (!(bits & 1u)) x.x = -INFINITY;
+                        if (!(bits & 2u)) x.y = -INFINITY;
+                        if (!(bits & 4u)) x.z = -INFINITY;
+                        if (!(bits & 8u)) x.w = -INFINITY;
                     }
-                    if (!(bits[u] & 1u)) x[u].x = -INFINITY;
-                    if (!(bits[u] & 2u)) x[u].y = -INFINITY;
-                    if (!(bits[u] & 4u)) x[u].z = -INFINITY;
-                    if (!(bits[u] & 8u)) x[u].w = -INFINITY;
-                    *reinterpret_cast<float4*>(p.out + (size_t)(c0 + row[u]) * p.vocab + t[u]) = x[u];
+                    *reinterpret_cast<float4*>(p.out + (size_t)(c0 + like + n * step) * p.vocab + t) = x;
+                };
+                auto counts_of = [&](int t, unsigned (&c)[4]) -> bool {
+                    if (!counted) return false;
+                    const int i = t - lo;
+                    if (!counts.wide && (i & 3) == 0) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(count_words + i / 2);
+                        if ((w.x | w.y) == 0u) return false;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[e] = counts.at(i + e);
+                    return (c[0] | c[1] | c[2] | c[3]) != 0u;
+                };
+                if (alike > 1) {                     // four rows' loads of a thread's four tokens together
+                    const int parts = (alike + 3) / 4;
+                    for (int i = threadIdx.x; i < fours * parts; i += NT) {
+                        const int part = i / fours, t = s0 + 4 * (i - part * fours), n0 = 4 * part;
+                        float4 x[4];
+                        unsigned bits[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) bits[u] = n0 + u < alike ? bits_of(n0 + u, t) : 0u;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (bits[u]) x[u] = __ldcg(reinterpret_cast<const float4*>(from(n0 + u) + t));
+                        }
+                        unsigned c[4] = {0u, 0u, 0u, 0u};
+                        const bool any = counts_of(t, c);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) if (n0 + u < alike) finish(x[u], bits[u], n0 + u, t, c, any);
+                    }
+                } else {                             // one row: a thread's loads of four fours
+                    for (int k0 = threadIdx.x; k0 < fours; k0 += 4 * NT) {
+                        float4 x[4];
+                        unsigned bits[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) bits[u] = k0 + u * NT < fours ? bits_of(0, s0 + 4 * (k0 + u * NT)) : 0u;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (bits[u]) x[u] = __ldcg(reinterpret_cast<const float4*>(from(0) + s0 + 4 * (k0 + u * NT)));
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            if (k0 + u * NT >= fours) continue;
+                            const int t = s0 + 4 * (k0 + u * NT);
+                            unsigned c[4] = {0u, 0u, 0u, 0u};
+                            const bool any = counts_of(t, c);
+                            finish(x[u], bits[u], 0, t, c, any);
+                        }
+                    }
                 }
             }
             // the up to three tokens of a row ahead of its fours, and those behind
@@ -184,33 +251,23 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
         }
         if (nodes > 0) {
             __syncthreads();
-            // the tokens of a node's path, a thread a node; one that is there more than once is done where the path has it first
-            for (int i = threadIdx.x; i < nodes; i += NT) {
-                int root = i;
-                while (root >= 0) root = parent[root];
-                if (root != -1) continue;            // padding, or a node behind it: no path
-                const size_t at = (size_t)(r0 + i) * p.vocab;
-                const int m = mask_of(r0 + i);
-                for (int a = i; a >= 0; a = parent[a]) {
-                    const int t = token[a];
-                    if (t < lo || t >= hi) continue;
-                    unsigned more = 1;
-                    bool first = true;
-                    for (int o = i; o > a; o = parent[o]) first = first && token[o] != t;
-                    for (int o = parent[a]; o >= 0; o = parent[o]) more += token[o] == t;
-                    if (!first) continue;
-                    const float x = penalised(__ldcg(p.logits + at + t), counts.at(t - lo), more, rep, freq, pres);
-                    p.out[at + t] = allowed(m, t) ? x : -INFINITY;
-                }
+            // a thread a node of the slice's and a node that may have it on its path; a token that is there more than once is done where
+            // the path has it first, for all of them
+            for (int i = threadIdx.x; i < hit_count * nodes; i += NT) {
+                const int a = hits[i / nodes], node = i % nodes, t = token[a];
+                int o = node;
+                bool first = true;
+                while (o > a) { first = first && token[o] != t; o = parent[o]; }
+                if (o != a || !first) continue;
+                unsigned more = 1;
+                for (o = parent[a]; o >= 0; o = parent[o]) more += token[o] == t;
+                if (o != -1) continue;               // padding, or a node behind it: no path
+                const size_t at = (size_t)(r0 + node) * p.vocab + t;
+                const float x = penalised(__ldcg(p.logits + at), counts.at(t - lo), more);
+                p.out[at] = allowed(mask_of(r0 + node), t) ? x : -INFINITY;
             }
         }
         if (biased) {
-            if (threadIdx.x == 0) { bias_range[0] = e1; bias_range[1] = e0; }
-            __syncthreads();
-            for (int e = e0 + threadIdx.x; e < e1; e += NT) {
-                const int t = p.bias_tokens[e];
-                if (t >= lo && t < hi) { atomicMin(&bias_range[0], e); atomicMax(&bias_range[1], e + 1); }
-            }
             __syncthreads();
             // ascending tokens: equal ones are neighbours, whose values the first of them adds in their order
             const int f0 = bias_range[0], f1 = bias_range[1], n = r1 - r0;
