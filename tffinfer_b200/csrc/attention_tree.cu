@@ -16,9 +16,11 @@
 #include "common.cuh"
 #include "attention_common.h"
 #include "attention_tree.cuh"
+#include "tma_host.h"
 
 namespace {
 
+constexpr float SLACK = 8.f;
 constexpr int BLOCK = 32, JOIN_THREADS = 128, NODE_WORDS = TREE_MAX_NODES / 32;
 
 struct TreeParams {
@@ -198,20 +200,23 @@ attention_tree_kernel(const T* q_in, const T* cache, T* __restrict__ out, const 
                 seen[j] = __ballot_sync(0xffffffffu, valid);
                 every &= seen[j];
                 s = valid ? s : -INFINITY;
-                const float mn = fmaxf(m[j], warp_max(s));
-                const float alpha = m[j] == -INFINITY ? (mn == -INFINITY ? 1.f : 0.f) : expf(m[j] - mn);
-                const float pr = valid && s != -INFINITY ? expf(s - mn) : 0.f;        // (a score of -infinity has no weight)
-                l[j] = l[j] * alpha + warp_sum(pr);
-                m[j] = mn;
-                if (alpha != 1.f) {
+                // The reference of the exponentials is moved only when a score passes it by more than SLACK (the weights stay below e^SLACK):
+                // a vote in place of five shuffles, and another five for the sum, which every lane keeps for its own keys.
+                if (__any_sync(0xffffffffu, s > m[j] + SLACK || (m[j] == -INFINITY && s > -INFINITY))) {
+                    const float mn = fmaxf(m[j], warp_max(s));
+                    const float alpha = m[j] == -INFINITY ? 0.f : expf(m[j] - mn);
+                    l[j] *= alpha;
+                    m[j] = mn;
 #pragma unroll
                     for (int c = 0; c < 4 * ND; ++c) o[j][c] *= alpha;
                 }
+                const float pr = valid && s != -INFINITY ? expf(s - m[j]) : 0.f;      // (a score of -infinity has no weight)
+                l[j] += pr;
                 sp[j * BLOCK + lane] = pr;
             }
             __syncwarp();
             // ------------------------------------------------ values: the lane's columns of the warp's rows
-#pragma unroll 1
+#pragma unroll 2
             for (int c = 0; c < BLOCK; c += 4) {
                 float4 x4[RW];
 #pragma unroll
@@ -245,6 +250,8 @@ attention_tree_kernel(const T* q_in, const T* cache, T* __restrict__ out, const 
         __syncthreads();
     }
 #pragma unroll
+    for (int j = 0; j < RW; ++j) l[j] = warp_sum(l[j]);
+#pragma unroll
     for (int j = 0; j < RW; ++j) {
         if (wrow + j >= rows) continue;
         const int h = kvh * G + (wrow + j) % G;
@@ -266,28 +273,36 @@ attention_tree_kernel(const T* q_in, const T* cache, T* __restrict__ out, const 
     }
 }
 
-// Joins the shares of a (node, head): a block each, a thread a column (of every JOIN_THREADS).
+// Joins the shares (32 at most) of a (node, head): a block each, a lane a share for the weights, a thread a column (of every JOIN_THREADS)
+// for the values, eight shares' loads together.
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS)
 attention_tree_join_kernel(T* __restrict__ out, const TreeParams p) {
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.y, t = blockIdx.x / p.nq, h = blockIdx.x % p.nq, q0 = p.q_start[b];
-    if (t >= p.q_start[b + 1] - q0) return;
+    const int b = blockIdx.y, t = blockIdx.x / p.nq, h = blockIdx.x % p.nq, q0 = p.q_start[b], lane = threadIdx.x & 31;
+    if (t >= min(p.q_start[b + 1] - q0, TREE_MAX_NODES)) return;
     const size_t item = (size_t)(q0 + t) * p.nq + h;
-    const float* ml = p.part_ml + item * p.splits * 2;
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, __ldcg(ml + 2 * s));
-    for (int s = 0; s < p.splits; ++s) {
-        const float ls = __ldcg(ml + 2 * s + 1);
-        if (ls > 0.f) l = fmaf(ls, expf(__ldcg(ml + 2 * s) - m), l);
-    }
+    const float2 ml = lane < p.splits ? __ldcg((const float2*)p.part_ml + item * p.splits + lane) : make_float2(-INFINITY, 0.f);
+    const float m = warp_max(ml.y > 0.f ? ml.x : -INFINITY);
+    const float f = ml.y > 0.f ? expf(ml.x - m) : 0.f;       // (a share that the row sees nothing of counts for nothing)
+    const float l = warp_sum(ml.y * f);
     const float inv = tree_weight(l, m, p.sink, p.sink_val, h) * (p.gate ? __ldcg(p.gate + item) : 1.f);
-    for (int col = threadIdx.x; col < p.dv; col += JOIN_THREADS) {
+    for (int col0 = 0; col0 < p.dv; col0 += JOIN_THREADS) {
+        const int col = col0 + threadIdx.x;
         float o = 0.f;
-        for (int s = 0; s < p.splits; ++s)
-            if (__ldcg(ml + 2 * s + 1) > 0.f) o = fmaf(__ldcg(p.part_o + (item * p.splits + s) * p.dv + col), expf(__ldcg(ml + 2 * s) - m), o);
-        out[item * p.dv + col] = from_f32<T>(l > 0.f ? o * inv : 0.f);
+        for (int s0 = 0; s0 < p.splits; s0 += 8) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                v[u] = s0 + u < p.splits && col < p.dv ? __ldcg(p.part_o + (item * p.splits + s0 + u) * p.dv + col) : 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float w = __shfl_sync(0xffffffffu, f, (s0 + u) & 31);
+                if (w > 0.f) o = fmaf(v[u], w, o);
+            }
+        }
+        if (col < p.dv) out[item * p.dv + col] = from_f32<T>(l > 0.f ? o * inv : 0.f);
     }
 }
 
@@ -314,9 +329,13 @@ template <typename T>
 int dispatch(const void* q, const void* cache, void* out, const TreeParams& p, int requests, int max_nodes, cudaStream_t s) {
     const int rows = max_nodes * (p.nq / p.nkv);
     int st;
+    // Tiles of 32 rows: 16 warps of two rows where there is at most a CTA an SM (26 rows a kv head behind 550 keys, two requests: 24 us, with
+    // 8 warps of four 29), else two CTAs of 8 warps (72 tiles behind 900: 75 us, with 16 warps 86).
+    const long long ctas = (long long)((rows + 31) / 32) * p.nkv * requests * p.splits;
     if (p.dv <= 128) st = rows <= 8 ? launch<T, 8, 1, 1>(q, cache, out, p, requests, max_nodes, s)
-                                    : rows <= 16 ? launch<T, 8, 2, 1>(q, cache, out, p, requests, max_nodes, s)
-                                                 : launch<T, 8, 4, 1>(q, cache, out, p, requests, max_nodes, s);
+                          : rows <= 16 ? launch<T, 8, 2, 1>(q, cache, out, p, requests, max_nodes, s)
+                          : ctas <= tff_num_sms() ? launch<T, 16, 2, 1>(q, cache, out, p, requests, max_nodes, s)
+                                                  : launch<T, 8, 4, 1>(q, cache, out, p, requests, max_nodes, s);
     else if (p.dv <= 256) st = launch<T, 8, 2, 2>(q, cache, out, p, requests, max_nodes, s);
     else st = launch<T, 8, 1, 4>(q, cache, out, p, requests, max_nodes, s);
     if (st == TFF_OK && p.splits > 1)
@@ -329,7 +348,7 @@ int tile_rows(int rows, int dv) { return dv <= 128 ? (rows <= 8 ? 8 : rows <= 16
 
 }  // namespace
 
-// In how many shares the general kernel's key blocks go to different CTAs: two CTAs an SM, at least 4 blocks a share.
+// In how many shares the general kernel's key blocks go to different CTAs: as many as fill the SMs, at least 2 blocks a share.
 // ``max_kv`` bounds the cached tokens and nodes of a request.  With s > 1 shares the call needs num_tokens * nq * s * (dv + 2) floats.
 TFF_API int tff_attention_tree_splits(int requests, int max_nodes, int max_kv, int nq, int nkv, int dv, int window, int keep, int sms) {
     if (requests <= 0 || max_nodes <= 0 || max_kv <= 0 || nkv <= 0 || nq <= 0 || nq % nkv || dv <= 0 || sms <= 0) return 1;
@@ -337,8 +356,10 @@ TFF_API int tff_attention_tree_splits(int requests, int max_nodes, int max_kv, i
     const long long ctas = (rows + tile - 1) / tile * nkv * requests;
     long long keys = max_kv;
     if (window > 0 && (long long)window + keep + max_nodes < keys) keys = (long long)window + keep + max_nodes;
-    long long s = 2ll * sms / ctas;
-    if (s > keys / (4 * BLOCK)) s = keys / (4 * BLOCK);
+    // a CTA an SM where that makes four shares or more (of 16 warps then: dispatch), else two
+    long long s = sms / ctas;
+    if (s < 4) s = 2ll * sms / ctas;
+    if (s > keys / (2 * BLOCK)) s = keys / (2 * BLOCK);
     if (s > 32) s = 32;
     return s < 1 || requests * s > 65535 ? 1 : (int)s;
 }

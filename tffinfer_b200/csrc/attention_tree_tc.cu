@@ -760,7 +760,7 @@ TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* 
                                   long long ws_floats, cudaStream_t stream) {
     if (num_tokens <= 0 || requests <= 0 || max_nodes <= 0) return TFF_OK;
     if (!q || !q_start || !pos_start || !parents || !block_table || !cache || !out || nq <= 0 || nkv <= 0 || nq % nkv || softcap < 0.f ||
-        keep < 0 || least <= 0 || extra < 0 || extra > 64 || table_width <= 0 || !ws)
+        keep < 0 || least <= 0 || extra < 0 || extra > 64 || table_width <= 0 || (!whole && !ws))
         return TFF_ERR_BAD_ARGUMENT;
     if ((d != 64 && d != 128) || (page_size != 8 && page_size != 16 && page_size != 32 && page_size != 64)) return TFF_ERR_UNSUPPORTED;
     if (nq / nkv > BLOCK_M) return TFF_ERR_UNSUPPORTED;          // a tile holds whole nodes
@@ -774,7 +774,7 @@ TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* 
     // (the line's units are counted in 32 bits)
     if ((((long long)table_width * page_size + TREE_MAX_NODES) / BLOCK_N + 2 + extra) * requests * nkv * ((long long)TREE_MAX_NODES * group / tile_rows + 1) >= (1ll << 31))
         return TFF_ERR_UNSUPPORTED;
-    if (ws_floats < (long long)sms * (4 + 2 * qt * BLOCK_M * (d + 2))) return TFF_ERR_BAD_ARGUMENT;
+    if (!whole && ws_floats < (long long)sms * (4 + 2 * qt * BLOCK_M * (d + 2))) return TFF_ERR_BAD_ARGUMENT;
     CUtensorMap tm, tq;
     if (!tff_tensor_map_kv_groups(cache, rows, d, page_size, nkv, &tm)) return TFF_ERR_DRIVER;
     if (!tff_tensor_map_heads(q, num_tokens, nkv, group, d, tile_rows / group, &tq)) return TFF_ERR_DRIVER;

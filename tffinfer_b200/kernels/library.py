@@ -888,14 +888,14 @@ class CudaKernels:
         c_ptr, c_pages, c_layers, c_layer = self._cache_args(kv_cache, kv_layer)
         sink_on, sink_val = self._sink_args(sink, nq)
         # a CTA's shares of two walks: rows of d values, a maximum and a sum; and which walk it ends
-        rows = 2 * self.NUM_SMS * (256 if batch.max_q_len * (nq // nkv) > 128 else 128)
-        ws = torch.empty(rows * (d + 2) + 4 * self.NUM_SMS, dtype=torch.float32, device=q.device)
+        floats = 0 if whole else self.NUM_SMS * (4 + 2 * (256 if batch.max_q_len * (nq // nkv) > 96 else 128) * (d + 2))
+        ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
         status = self.lib.tff_attention_tree_tc(
             _ptr(q), _ptr(batch.q_start), _ptr(batch.pos_start), _ptr(parents), _ptr(block_table), _c_int(block_table.shape[1]),
             c_ptr, _c_int(c_pages), _c_int(c_layers), _c_int(c_layer), _c_int(page_size), _ptr(out), _c_int(T), _c_int(B),
             _c_int(batch.max_q_len), _c_int(nq), _c_int(nkv), _c_int(d), _c_float(scale), _c_int(window), _c_float(softcap),
             _c_int(1 if sink_on else 0), _ptr(sink_val), _ptr(gates), _c_int(keep), _c_int(least), _c_int(extra), _c_int(1 if whole else 0), _ptr(ws),
-            _c_int(ws.numel()),
+            _c_int(floats),
             self._stream())
         if status == -2:
             return False
