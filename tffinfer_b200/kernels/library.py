@@ -829,7 +829,7 @@ class CudaKernels:
                                        softcap, sink, gates, keep)
 
     TREE_MAX_NODES = 256          # of a request's tree of drafted tokens
-    TREE_WHOLE_BLOCKS = 8         # up to so many blocks of 64 keys a request's walk is not divided
+    TREE_WHOLE_BLOCKS = 12        # up to so many blocks of 64 keys a request's walk is not divided
 
     def _tree_args(self, batch, parents, T: int, *others) -> None:
         """Checks what the kernels of drafted trees are given of a step, and ``others``, which are int32 as well."""
@@ -878,7 +878,7 @@ class CudaKernels:
                                    softcap, sink, gates, keep)
 
     def _attention_tree_tc(self, q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, scale, window,
-                           softcap, sink, gates, keep, least: int = 4, extra: int = 3, whole=None) -> bool:
+                           softcap, sink, gates, keep, least: int = 4, extra: int = 6, whole=None) -> bool:
         """On the tensor cores; False, and nothing launched, for what that kernel does not take.  ``least``: blocks of 64 keys that
         a CTA's share has at least; ``extra``: how many of them a piece of a walk costs beside its own; ``whole``: shares are whole walks (None: where none has more than WHOLE_BLOCKS)."""
         T, B = q.shape[0], batch.num_requests
