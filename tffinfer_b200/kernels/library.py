@@ -37,6 +37,8 @@ def _c_float(x) -> float:
 
 
 _vp = ctypes.c_void_p
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else (lambda: 0)
+_I32, _F32 = torch.int32, torch.float32
 
 _STATUS = {
     -1: "bad argument (a size or pointer the kernel cannot take)",
@@ -183,11 +185,11 @@ class CudaKernels:
                 raise KernelError("kernels take contiguous tensors")
 
     @staticmethod
-    def _need_here(dtype, *tensors) -> None:
-        """Contiguous tensors of the type ``dtype`` (None: of any) on the current device, whose stream the launch goes to."""
-        here = torch._C._cuda_getDevice()
+    def _need_here(dtype, tensors) -> None:
+        """Contiguous tensors of the type ``dtype`` on the current device, whose stream the launch goes to; None is passed over."""
+        here = _current_device()
         for t in tensors:
-            if t is None or (t.get_device() == here and (dtype is None or t.dtype is dtype) and t.is_contiguous()):
+            if t is None or (t.dtype is dtype and t.get_device() == here and t.is_contiguous()):
                 continue
             CudaKernels._need_cuda(t)
             if t.get_device() != here:
@@ -831,13 +833,12 @@ class CudaKernels:
     TREE_MAX_NODES = 256          # of a request's tree of drafted tokens
     TREE_WHOLE_BLOCKS = 12        # up to so many blocks of 64 keys a request's walk is not divided
 
-    def _tree_args(self, batch, parents, T: int, *others) -> None:
-        """Checks what the kernels of drafted trees are given of a step, and ``others``, which are int32 as well."""
-        q_start, pos_start, B = batch.q_start, batch.pos_start, batch.num_requests
-        self._need_here(torch.int32, parents, q_start, pos_start, *others)
+    def _tree_args(self, batch, parents, T: int) -> None:
+        """Checks the sizes of what the kernels of drafted trees are given of a step."""
+        B = batch.num_requests
         if parents.numel() != T:
             raise KernelError(f"parents are {T} numbers, one a node")
-        if q_start.numel() <= B or pos_start.numel() < B:
+        if batch.q_start.numel() <= B or batch.pos_start.numel() < B:
             raise KernelError("q_start and pos_start have an element a request, and q_start one more")
         if batch.max_q_len > self.TREE_MAX_NODES:
             raise KernelError(f"a request brings at most {self.TREE_MAX_NODES} nodes, got {batch.max_q_len}")
@@ -854,14 +855,15 @@ class CudaKernels:
         ancestors (the queries and keys are rotated by it: ``batch.positions`` of such a step).  At most 256 nodes a request."""
         T, B, dtype = q.shape[0], batch.num_requests, q.dtype
         dc = kv_cache.shape[-1]
-        self._need_here(dtype, q, out)
-        self._tree_args(batch, parents, T, block_table)
+        self._need_here(dtype, (q, out))
+        self._need_here(_I32, (parents, batch.q_start, batch.pos_start, block_table))
+        self._tree_args(batch, parents, T)
         if kv_cache.dtype is not dtype or kv_cache.get_device() != q.get_device():
             raise KernelError("queries, cache and outputs have one type and lie on one device")
         if q.shape != (T, nq * d) or out.shape != (T, nq * dv) or kv_cache.shape[2:] != (2, nkv, page_size, dc) or dc < max(d, dv):
             raise KernelError("queries are [T, nq * d], outputs [T, nq * dv], cache pages [2, nkv, page, at least d and dv]")
         if gates is not None:
-            self._need_here(torch.float32, gates)
+            self._need_here(_F32, (gates,))
             if gates.shape != (T, nq):
                 raise KernelError("head gates are [T, nq]")
         if block_table.dim() != 2 or block_table.shape[0] < B:
@@ -930,7 +932,8 @@ class CudaKernels:
         both -1 beyond; count int32 [B]: their number (0 for a request without nodes)."""
         tokens = batch.token_ids
         T, B = tokens.numel(), batch.num_requests
-        self._tree_args(batch, parents, T, tokens, drawn, path, emitted, count)
+        self._need_here(_I32, (tokens, parents, drawn, path, emitted, count, batch.q_start, batch.pos_start))
+        self._tree_args(batch, parents, T)
         if drawn.numel() != T or path.dim() != 2 or path.shape[0] != B or path.shape != emitted.shape or count.numel() != B:
             raise KernelError("a draw a node, and path and emitted [requests, width], count [requests]")
         if B == 0 or path.shape[1] == 0:
@@ -946,7 +949,7 @@ class CudaKernels:
         [pages, layers, planes, kv heads, page, head]: slot pos_start[b] + path[b, j] to slot pos_start[b] + j, j < count[b].
         path and count as ``accept_tree`` gives them (a path's nodes ascend); the slots behind stay as they are."""
         B = batch.num_requests
-        self._need_here(torch.int32, block_table, path, count, batch.pos_start)
+        self._need_here(_I32, (block_table, path, count, batch.pos_start))
         if kv_cache.dim() != 6 or kv_cache.shape[4] != page_size:
             raise KernelError("the cache is [pages, layers, planes, kv heads, page, head]")
         if kv_cache.get_device() != path.get_device():
@@ -2398,9 +2401,9 @@ class CudaKernels:
         """out = logits (float32 [R, V]) under ``controls`` (sampling.LogitControls): penalties for repeated tokens, biases,
         grammar masks.  ``out`` may be ``logits`` itself unless the rows are nodes of trees."""
         c = controls
-        self._need_here(torch.float32, logits, out, c.settings, c.bias_values)
-        self._need_here(torch.int32, c.row_start, c.history, c.history_start, c.history_len, c.prompt_len, c.bias_start, c.bias_tokens,
-                        c.mask, c.mask_row, c.parents, c.tokens)
+        self._need_here(_F32, (logits, out, c.settings, c.bias_values))
+        self._need_here(_I32, (c.row_start, c.history, c.history_start, c.history_len, c.prompt_len, c.bias_start, c.bias_tokens, c.mask,
+                               c.mask_row, c.parents, c.tokens))
         R, V = logits.shape
         if out.shape != logits.shape:
             raise KernelError("logits and outputs are [rows, vocabulary]")
