@@ -11,8 +11,12 @@
 //
 // A CTA takes a slice of the vocabulary for all rows of one request: it counts the history's tokens of its slice in shared
 // memory (integers: in any order), once for all rows, and then streams the rows' slices, four logits a load and four loads a
-// thread on their way, of four rows where there are as many.  The few tokens of a row's path and the few biased ones are put right behind that pass, by the
-// same CTA.  Where a mask allows none of a load's four tokens nothing is read.
+// thread on their way, of four rows where there are as many.  What bounds it beside the traffic is instructions: a thread's
+// addresses are a pointer and an offset, and what a count does to a logit is worked out once for four rows, and not at all where none of a
+// thread's four tokens was seen (looked up and divided for every logit, 140 to 230 instructions for a warp's 128 of them, 256 rows of
+// trees took 62 us and 64 rows 30).  The few tokens of a row's path and the few biased ones are put right behind that pass.  Where a
+// mask allows none of a load's four tokens nothing is read.  Tried without gain: counted tokens put right behind a pass that only copies
+// (98 us and 34), parts of rows by bulk copies through shared memory (75 and 41: half the instructions, too few warps).
 #include "common.cuh"
 #include "tma_host.h"
 
@@ -21,8 +25,8 @@ namespace {
 constexpr int NT = 256, CTAS_AN_SM = 4;
 constexpr int MAX_NODES = 256;                       // of a request's tree
 constexpr int ROWS_AT_ONCE = 256;
-constexpr int MOST_TOKENS = 16384, LEAST_TOKENS = 1024;        // of a slice: 32 KB of counts leave room for four CTAs an SM
-constexpr int MASK_WORDS = 2048;                     // of masks in shared memory: a part of the rows' at a time
+constexpr int MOST_TOKENS = 12288, LEAST_TOKENS = 1024;        // of a slice: 24 KB of counts beside the rest's 20 leave room for four CTAs an SM
+constexpr int MASK_WORDS = 2304;                     // of masks in shared memory: a part of the rows' at a time
 
 struct ControlParams {
     const float* logits; float* out;
@@ -39,13 +43,15 @@ struct ControlParams {
 struct Counts {
     unsigned* words;
     bool wide;
-    __device__ __forceinline__ void prompt(int i) {
-        if (wide) atomicOr(words + i, 0x80000000u);
-        else atomicOr(words + (i >> 1), 0x8000u << (i & 1) * 16);
-    }
-    __device__ __forceinline__ void add(int i) {
-        if (wide) atomicAdd(words + i, 1u);
-        else atomicAdd(words + (i >> 1), 1u << (i & 1) * 16);
+    __device__ __forceinline__ void add(int i, bool prompt) const {
+        if (wide) {
+            if (prompt) atomicOr(words + i, 0x80000000u);
+            else atomicAdd(words + i, 1u);
+        } else {
+            const int shift = (i & 1) * 16;
+            if (prompt) atomicOr(words + (i >> 1), 0x8000u << shift);
+            else atomicAdd(words + (i >> 1), 1u << shift);
+        }
     }
     // (a count's top bit as the top bit of 32)
     __device__ __forceinline__ unsigned at(int i) const {
@@ -55,15 +61,21 @@ struct Counts {
     }
 };
 
-// A request's penalties.  A positive logit is multiplied by 1 / repetition, rounded once for the request: a second rounding in
-// float32 (2^-24) in place of a division, which with its branches took most of the kernel's instructions.
+// A request's penalties.  A positive logit of a token that was seen is multiplied by 1 / repetition, rounded once for the request: a second
+// rounding in float32 (2^-24) in place of a division an element.
 struct Penalties {
     float rep, inverse, freq, pres;
-    // ``count`` as Counts gives it; ``more`` times on the row's path.  What was not seen keeps its bits.
+    // What is added to the logit of a token with this count (as Counts gives it): -0, which leaves all bits, where it was not generated.
+    __device__ __forceinline__ float less(unsigned count) const {
+        const unsigned n = count & 0x7fffffffu;
+        return n ? -fmaf(freq, (float)n, pres) : -0.f;
+    }
+    __device__ __forceinline__ float apply(float x, bool seen, float less_) const {
+        return fmaf(x, seen ? x > 0.f ? inverse : rep : 1.f, less_);
+    }
+    // ``more`` times on the row's path.
     __device__ __forceinline__ float operator()(float x, unsigned count, unsigned more = 0u) const {
-        const unsigned n = (count & 0x7fffffffu) + more;
-        const float factor = (count | more) == 0u ? 1.f : x > 0.f ? inverse : rep;
-        return x * factor - (n ? fmaf(freq, (float)n, pres) : 0.f);
+        return apply(x, (count | more) != 0u, less((count & 0x7fffffffu) + more));
     }
 };
 
@@ -73,90 +85,117 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
     extern __shared__ unsigned count_words[];        // [slice / 2]
     __shared__ int mask_at[ROWS_AT_ONCE];
     __shared__ unsigned masks[MASK_WORDS];           // of a part of the rows: [row][words of the slice]
-    __shared__ short hits[MAX_NODES];                // nodes whose tokens lie in the slice
-    __shared__ int hit_count;
     __shared__ short parent[MAX_NODES];
     __shared__ int token[MAX_NODES];
-    __shared__ int bias_range[2];                    // of the slice
+    __shared__ unsigned short lists[NT / 32][512];   // a warp's tokens of the slice: their places, and a bit for the prompt's
+    __shared__ short hits[MAX_NODES];                // nodes whose tokens lie in the slice
+    __shared__ int hit_count, bias_range[2];
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.y;
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+    // (all on their way together)
     const int r0 = max(0, p.row_start[b]), r1 = min(p.rows, p.row_start[b + 1]);
-    if (r0 >= r1) return;
     Penalties penalised;
     penalised.rep = p.settings[3 * b]; penalised.freq = p.settings[3 * b + 1]; penalised.pres = p.settings[3 * b + 2];
+    const long long first_token = p.history_start[b], held = p.history_len[b];
+    const int prompt = p.prompt_len[b];
+    const int e0 = p.bias_start ? max(0, p.bias_start[b]) : 0, e1 = p.bias_start ? min(p.biases, p.bias_start[b + 1]) : 0;
+    if (r0 >= r1) return;
     penalised.inverse = 1.f / penalised.rep;
     const bool counted = penalised.rep != 1.f || penalised.freq != 0.f || penalised.pres != 0.f;
-    const long long first_token = p.history_start[b];
-    const int len = first_token < 0 ? 0 : (int)max(0ll, min((long long)p.history_len[b], p.history_size - first_token));
-    const int prompt = p.prompt_len[b];
+    const int len = !counted || first_token < 0 ? 0 : (int)max(0ll, min(held, p.history_size - first_token));
     Counts counts;
     counts.words = count_words;
     counts.wide = len > 32767;
-    const int e0 = p.bias_start ? max(0, p.bias_start[b]) : 0, e1 = p.bias_start ? min(p.biases, p.bias_start[b + 1]) : 0;
-    const bool biased = e0 < e1;
     const int nodes = p.parents && counted ? min(r1 - r0, MAX_NODES) : 0;
-    for (int i = threadIdx.x; i < nodes; i += NT) {
+    for (int i = tid; i < nodes; i += NT) {
         const int up = __ldcg(p.parents + r0 + i);
         parent[i] = (short)(up < -1 || up >= i ? -2 : up);
         token[i] = __ldcg(p.tokens + r0 + i);
     }
-    auto allowed = [&](int m, int t) { return m < 0 || (__ldcg(p.mask + (size_t)m * p.mask_words + (t >> 5)) >> (t & 31) & 1u); };
     auto mask_of = [&](int r) {
         const int m = p.mask ? (p.mask_row ? __ldcg(p.mask_row + r) : r) : -1;
         return m < p.mask_rows ? m : -1;
     };
+    auto allowed = [&](int r, int t) {
+        const int m = mask_of(r);
+        return m < 0 || (__ldcg(p.mask + (size_t)m * p.mask_words + (t >> 5)) >> (t & 31) & 1u);
+    };
     const int end = min(p.vocab, (int)(blockIdx.x + 1) * p.slice), width = counts.wide ? p.slice / 2 : p.slice;
     for (int lo = blockIdx.x * p.slice; lo < end; lo += width) {
         const int hi = min(end, lo + width);
+        const int w0 = lo >> 5, words = ((hi - 1) >> 5) - w0 + 1;
+        // rows at a time: in equal parts, of whole fours
+        const int most = p.mask ? min(ROWS_AT_ONCE, MASK_WORDS / words) : ROWS_AT_ONCE, parts = (r1 - r0 + most - 1) / most;
+        const int at_once = min(most, ((r1 - r0 + parts - 1) / parts + 3) & ~3);
         __syncthreads();                             // (the part before is through with the counts)
-        if (counted) {
-            for (int i = threadIdx.x; i < p.slice / 2; i += NT) count_words[i] = 0u;
-            __syncthreads();
-            for (int i0 = threadIdx.x; i0 < len; i0 += 8 * NT) {
-                int t[8];
+        if (len > 0) for (int i = tid; i < p.slice / 8; i += NT) reinterpret_cast<uint4*>(count_words)[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (tid == 0) { hit_count = 0; bias_range[0] = e1; bias_range[1] = e0; }
+        __syncthreads();
+        // Four tokens a load, from the 16 bytes on in which the history begins.  Few of them are the slice's: a warp lists those of its
+        // 512 tokens and then counts them a lane each.  (With a branch for every token nearly every one was taken by some lane.)
+        const int* at = p.history + first_token;
+        const int skew = (int)((uintptr_t)at >> 2 & 3), warp0 = tid & ~31;
+        unsigned short* list = lists[tid >> 5];
+        for (int g0 = 0; (g0 + warp0) * 4 - skew < len; g0 += 4 * NT) {
+            int4 t4[4];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) t[u] = i0 + u * NT < len ? __ldcg(p.history + first_token + i0 + u * NT) : -1;
+            for (int u = 0; u < 4; ++u) {
+                const int g = g0 + u * NT + tid;
+                t4[u] = make_int4(-1, -1, -1, -1);
+                if (g * 4 - skew < len) t4[u] = __ldcg(reinterpret_cast<const int4*>(at - skew) + g);
+            }
+            int n = 0;
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    if (t[u] < lo || t[u] >= hi) continue;
-                    if (i0 + u * NT < prompt) counts.prompt(t[u] - lo);
-                    else counts.add(t[u] - lo);
+            for (int u = 0; u < 4; ++u) {
+                const int t[4] = {t4[u].x, t4[u].y, t4[u].z, t4[u].w};
+                const int i0 = (g0 + u * NT + tid) * 4 - skew;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned place = (unsigned)(t[e] - lo);
+                    const bool hit = place < (unsigned)(hi - lo) && (unsigned)(i0 + e) < (unsigned)len;
+                    const unsigned found = __ballot_sync(0xffffffffu, hit);
+                    if (hit) list[n + __popc(found & ((1u << lane) - 1))] = (unsigned short)(place | (i0 + e < prompt ? 0x8000u : 0u));
+                    n += __popc(found);
                 }
             }
+            __syncwarp();
+            for (int i = lane; i < n; i += 32) counts.add(list[i] & 0x7fff, list[i] >> 15);
+            __syncwarp();
         }
-        // the biases of the slice: a run of the request's
-        if (threadIdx.x == 0) { bias_range[0] = e1; bias_range[1] = e0; hit_count = 0; }
-        __syncthreads();
-        for (int e = e0 + threadIdx.x; e < e1; e += NT) {
+        for (int e = e0 + tid; e < e1; e += NT) {
             const int t = p.bias_tokens[e];
             if (t >= lo && t < hi) { atomicMin(&bias_range[0], e); atomicMax(&bias_range[1], e + 1); }
         }
-        for (int i = threadIdx.x; i < nodes; i += NT)
+        for (int i = tid; i < nodes; i += NT)
             if (token[i] >= lo && token[i] < hi) hits[atomicAdd(&hit_count, 1)] = (short)i;
-        const int w0 = lo >> 5, words = ((hi - 1) >> 5) - w0 + 1;
-        const int at_once = p.mask ? min(ROWS_AT_ONCE, MASK_WORDS / words) : ROWS_AT_ONCE;
+
+        // ------------------------------------------------ the rows' slices
         for (int c0 = r0; c0 < r1; c0 += at_once) {
             const int rows = min(at_once, r1 - c0);
-            if (c0 > r0) __syncthreads();
-            for (int i = threadIdx.x; i < rows; i += NT) mask_at[i] = mask_of(c0 + i);
-            __syncthreads();
+            bool masked = false;
             if (p.mask) {
-                for (int i = threadIdx.x; i < rows * words; i += NT) {
-                    const int m = mask_at[i / words];
-                    masks[i] = m < 0 ? 0xffffffffu : __ldcg(p.mask + (size_t)m * p.mask_words + w0 + i % words);
+                if (c0 > r0) __syncthreads();
+                for (int i = tid; i < rows; i += NT) { mask_at[i] = mask_of(c0 + i); masked = masked || mask_at[i] >= 0; }
+                masked = __syncthreads_or(masked);
+                if (masked) {
+                    for (int i = tid; i < rows * words; i += NT) {
+                        const int m = mask_at[i / words];
+                        masks[i] = m < 0 ? 0xffffffffu : __ldcg(p.mask + (size_t)m * p.mask_words + w0 + i % words);
+                    }
+                    __syncthreads();
                 }
+            } else if (c0 == r0) {
                 __syncthreads();
             }
-            auto allowed_here = [&](int row, int t) { return !p.mask || (masks[row * words + (t >> 5) - w0] >> (t & 31) & 1u); };
             auto one = [&](int row, int t) {
-                const size_t at = (size_t)(c0 + row) * p.vocab + t;
-                const float x = __ldcg(p.logits + at);
-                p.out[at] = allowed_here(row, t) ? penalised(x, counted ? counts.at(t - lo) : 0u) : -INFINITY;
+                const size_t i = (size_t)(c0 + row) * p.vocab + t;
+                const float x = penalised(__ldcg(p.logits + i), len > 0 ? counts.at(t - lo) : 0u);
+                p.out[i] = masked && !(masks[row * words + (t >> 5) - w0] >> (t & 31) & 1u) ? -INFINITY : x;
             };
             if (!VEC) {
                 for (int row = 0; row < rows; ++row)
-                    for (int t = lo + threadIdx.x; t < hi; t += NT) one(row, t);
+                    for (int t = lo + tid; t < hi; t += NT) one(row, t);
                 continue;
             }
             // tokens ahead of a row's first aligned four: the same for every fourth row, and for all where vocab is a multiple of 4
@@ -166,113 +205,140 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
             const int step = p.vocab & 3 ? 4 : 1;
             for (int like = 0; like < min(step, rows); ++like) {
                 const int s0 = lo + skip(like), fours = (hi - s0) / 4, alike = (rows - like + step - 1) / step;
-                auto from = [&](int n) { return p.logits + (size_t)(c0 + like + n * step) * p.vocab; };
-                auto bits_of = [&](int n, int t) -> unsigned {
-                    if (!p.mask) return 15u;
-                    const unsigned* w = masks + (like + n * step) * words + (t >> 5) - w0;
-                    const unsigned low = w[0], high = (t & 31) > 28 ? w[1] : 0u;
-                    return __funnelshift_r(low, high, t & 31) & 15u;
+                const size_t row0 = (size_t)(c0 + like) * p.vocab + s0;
+                const float4* from = reinterpret_cast<const float4*>(p.logits + row0);           // of the fours' first row
+                float4* to = reinterpret_cast<float4*>(p.out + row0);
+                const int pitch = p.vocab / 4 * step + (p.vocab & 3) * (step / 4);                // fours from a row to the next that is alike
+                const unsigned* bits_at = masks + like * words;
+                const int bits_pitch = step * words, bit0 = s0 - 32 * w0;
+                auto bits_of = [&](int n, int k) -> unsigned {
+                    const int at = bit0 + 4 * k;
+                    const unsigned* w = bits_at + n * bits_pitch + (at >> 5);
+                    return __funnelshift_r(w[0], (at & 31) > 28 ? w[1] : 0u, at & 31) & 15u;
                 };
-                auto finish = [&](float4 x, unsigned bits, int n, int t, const unsigned (&c)[4], bool any) {
-                    if (any) {
-                        x.x = penalised(x.x, c[0]);
-                        x.y = penalised(x.y, c[1]);
-                        x.z = penalised(x.z, c[2]);
-                        x.w = penalised(x.w, c[3]);
-                    }
-                    if (bits != 15u) {
-                        if (!(bits & 1u)) x.x = -INFINITY;
-                        if (!(bits & 2u)) x.y = -INFINITY;
-                        if (!(bits & 4u)) x.z = -INFINITY;
-                        if (!(bits & 8u)) x.w = -INFINITY;
-                    }
-                    *reinterpret_cast<float4*>(p.out + (size_t)(c0 + like + n * step) * p.vocab + t) = x;
-                };
-                auto counts_of = [&](int t, unsigned (&c)[4]) -> bool {
-                    if (!counted) return false;
-                    const int i = t - lo;
-                    if (!counts.wide && (i & 3) == 0) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(count_words + i / 2);
-                        if ((w.x | w.y) == 0u) return false;
-                    }
+                // Which of the thread's four tokens were seen (a bit each), and what is added to their logits.
+                const bool aligned = !counts.wide && ((s0 - lo) & 3) == 0;
+                const uint2* pairs = reinterpret_cast<const uint2*>(count_words) + (s0 - lo) / 4;
+                auto seen_of = [&](int k, float (&less)[4]) -> unsigned {
+                    if (len == 0) return 0u;
+                    unsigned c[4];
+                    if (aligned) {
+                        const uint2 w = pairs[k];
+                        if ((w.x | w.y) == 0u) return 0u;
+                        c[0] = w.x & 0xffffu; c[1] = w.x >> 16; c[2] = w.y & 0xffffu; c[3] = w.y >> 16;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) c[e] = counts.at(i + e);
-                    return (c[0] | c[1] | c[2] | c[3]) != 0u;
+                        for (int e = 0; e < 4; ++e) less[e] = penalised.less(c[e] & 0x7fffu);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) { c[e] = counts.at(s0 - lo + 4 * k + e); less[e] = penalised.less(c[e]); }
+                    }
+                    return (c[0] ? 1u : 0u) | (c[1] ? 2u : 0u) | (c[2] ? 4u : 0u) | (c[3] ? 8u : 0u);
                 };
-                if (alike > 1) {                     // four rows' loads of a thread's four tokens together
-                    const int parts = (alike + 3) / 4;
-                    for (int i = threadIdx.x; i < fours * parts; i += NT) {
-                        const int part = i / fours, t = s0 + 4 * (i - part * fours), n0 = 4 * part;
+                auto penalise = [&](float4& x, unsigned seen, const float (&less)[4]) {
+                    x.x = penalised.apply(x.x, seen & 1u, less[0]); x.y = penalised.apply(x.y, seen & 2u, less[1]);
+                    x.z = penalised.apply(x.z, seen & 4u, less[2]); x.w = penalised.apply(x.w, seen & 8u, less[3]);
+                };
+                auto ban = [&](float4& x, unsigned bits) {
+                    if (!(bits & 1u)) x.x = -INFINITY;
+                    if (!(bits & 2u)) x.y = -INFINITY;
+                    if (!(bits & 4u)) x.z = -INFINITY;
+                    if (!(bits & 8u)) x.w = -INFINITY;
+                };
+                if (alike > 1) {                     // a thread's four tokens in four rows
+                    const int turns = (alike + 3) / 4;
+                    for (int j = tid; j < fours * turns; j += NT) {
+                        const int turn = j / fours, k = j - turn * fours, n0 = 4 * turn, left = alike - n0;
+                        const float4* src = from + (size_t)n0 * pitch + k;
+                        float4* dst = to + (size_t)n0 * pitch + k;
                         float4 x[4];
-                        unsigned bits[4];
+                        unsigned bits = 0xffffu;     // of the four rows
+                        if (masked) {
+                            bits = 0u;
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) bits[u] = n0 + u < alike ? bits_of(n0 + u, t) : 0u;
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (bits[u]) x[u] = __ldcg(reinterpret_cast<const float4*>(from(n0 + u) + t));
+                            for (int u = 0; u < 4; ++u) if (u < left) bits |= bits_of(n0 + u, k) << (4 * u);
                         }
-                        unsigned c[4] = {0u, 0u, 0u, 0u};
-                        const bool any = counts_of(t, c);
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) if (n0 + u < alike) finish(x[u], bits[u], n0 + u, t, c, any);
-                    }
-                } else {                             // one row: a thread's loads of four fours
-                    for (int k0 = threadIdx.x; k0 < fours; k0 += 4 * NT) {
-                        float4 x[4];
-                        unsigned bits[4];
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) bits[u] = k0 + u * NT < fours ? bits_of(0, s0 + 4 * (k0 + u * NT)) : 0u;
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
                             x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (bits[u]) x[u] = __ldcg(reinterpret_cast<const float4*>(from(0) + s0 + 4 * (k0 + u * NT)));
+                            if (u < left && (bits >> (4 * u) & 15u)) x[u] = __ldcg(src + u * pitch);
+                        }
+                        float less[4];
+                        const unsigned seen = seen_of(k, less);
+                        if (seen) {
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) penalise(x[u], seen, less);
+                        }
+                        if (bits != 0xffffu) {
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) ban(x[u], bits >> (4 * u));
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) if (u < left) dst[u * pitch] = x[u];
+                    }
+                } else {                             // 16 tokens of a row
+                    for (int k0 = tid; k0 < fours; k0 += 4 * NT) {
+                        float4 x[4];
+                        unsigned bits = 0xffffu;
+                        if (masked) {
+                            bits = 0u;
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) if (k0 + u * NT < fours) bits |= bits_of(0, k0 + u * NT) << (4 * u);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (k0 + u * NT < fours && (bits >> (4 * u) & 15u)) x[u] = __ldcg(from + k0 + u * NT);
                         }
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
                             if (k0 + u * NT >= fours) continue;
-                            const int t = s0 + 4 * (k0 + u * NT);
-                            unsigned c[4] = {0u, 0u, 0u, 0u};
-                            const bool any = counts_of(t, c);
-                            finish(x[u], bits[u], 0, t, c, any);
+                            float less[4];
+                            const unsigned seen = seen_of(k0 + u * NT, less);
+                            if (seen) penalise(x[u], seen, less);
+                            if (bits != 0xffffu) ban(x[u], bits >> (4 * u));
+                            to[k0 + u * NT] = x[u];
                         }
                     }
                 }
             }
             // the up to three tokens of a row ahead of its fours, and those behind
-            for (int i = threadIdx.x; i < rows * 6; i += NT) {
-                const int row = i / 6, e = i % 6, s = skip(row), left = (hi - lo - s) & 3;
-                if (hi - lo < s) {                   // (a slice of fewer tokens than that)
-                    if (e < hi - lo) one(row, lo + e);
-                } else if (e < 3 ? e < s : e - 3 < left) {
-                    one(row, e < 3 ? lo + e : hi - left + e - 3);
+            if (p.vocab & 3 || ((uintptr_t)p.logits & 15) || ((hi - lo) & 3)) {
+                for (int i = tid; i < rows * 6; i += NT) {
+                    const int row = i / 6, e = i % 6, s = skip(row), left = (hi - lo - s) & 3;
+                    if (hi - lo < s) {               // (a slice of fewer tokens than that)
+                        if (e < hi - lo) one(row, lo + e);
+                    } else if (e < 3 ? e < s : e - 3 < left) {
+                        one(row, e < 3 ? lo + e : hi - left + e - 3);
+                    }
                 }
             }
         }
+
+        // ------------------------------------------------ what paths and biases change
         if (nodes > 0) {
             __syncthreads();
             // a thread a node of the slice's and a node that may have it on its path; a token that is there more than once is done where
             // the path has it first, for all of them
-            for (int i = threadIdx.x; i < hit_count * nodes; i += NT) {
-                const int a = hits[i / nodes], node = i % nodes, t = token[a];
+            for (int i = tid; i < hit_count * nodes; i += NT) {
+                const int up = hits[i / nodes], node = i % nodes, t = token[up];
                 int o = node;
                 bool first = true;
-                while (o > a) { first = first && token[o] != t; o = parent[o]; }
-                if (o != a || !first) continue;
+                while (o > up) { first = first && token[o] != t; o = parent[o]; }
+                if (o != up || !first) continue;
                 unsigned more = 1;
-                for (o = parent[a]; o >= 0; o = parent[o]) more += token[o] == t;
+                for (o = parent[up]; o >= 0; o = parent[o]) more += token[o] == t;
                 if (o != -1) continue;               // padding, or a node behind it: no path
-                const size_t at = (size_t)(r0 + node) * p.vocab + t;
-                const float x = penalised(__ldcg(p.logits + at), counts.at(t - lo), more);
-                p.out[at] = allowed(mask_of(r0 + node), t) ? x : -INFINITY;
+                const size_t k = (size_t)(r0 + node) * p.vocab + t;
+                const float x = __ldcg(p.logits + k);
+                if (allowed(r0 + node, t)) p.out[k] = penalised(x, len > 0 ? counts.at(t - lo) : 0u, more);
             }
         }
-        if (biased) {
+        const int f0 = bias_range[0], f1 = bias_range[1], n_rows = r1 - r0;
+        if (f0 < f1) {
             __syncthreads();
             // ascending tokens: equal ones are neighbours, whose values the first of them adds in their order
-            const int f0 = bias_range[0], f1 = bias_range[1], n = r1 - r0;
-            for (long long i = threadIdx.x; i < (long long)(f1 - f0) * n; i += NT) {
-                const int e = f0 + (int)(i / n), r = r0 + (int)(i % n);
+            for (long long i = tid; i < (long long)(f1 - f0) * n_rows; i += NT) {
+                const int e = f0 + (int)(i / n_rows), r = r0 + (int)(i % n_rows);
                 const int t = p.bias_tokens[e];
                 if (t < lo || t >= hi || (e > e0 && p.bias_tokens[e - 1] == t)) continue;
                 float bias = p.bias_values[e];
@@ -284,8 +350,7 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
     }
 }
 
-// Tokens of a slice: as many slices a request as fill whole waves of four CTAs an SM, of few tokens where there are few
-// requests.
+// Tokens of a slice: as many slices a request as fill whole waves, of few tokens where there are few requests.
 int slice_tokens(int vocab, int requests, int sms) {
     const long long slots = (long long)CTAS_AN_SM * (sms > 0 ? sms : 1);
     for (int wave = 1;; ++wave) {
