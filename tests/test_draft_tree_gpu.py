@@ -312,11 +312,12 @@ def test_slots_of_paths_that_are_none(ops):
     path, count = i32([[0, 500, -3, 1 << 30], [0, 6, 7, 8], [0, 5, 6, 9]]), i32([99, 4, 4])
     ops.keep_path(cache, batch, table, 8, path, count)
     assert torch.equal(cache, before)
-    for bad in (dict(path=path[:2]), dict(count=count[:2]), dict(path=path.long()), dict(page=16), dict(table=table[:2])):
-        a = dict(table=table, page=8, path=path, count=count)
+    for bad in (dict(path=path[:2]), dict(count=count[:2]), dict(path=path.long()), dict(page=16), dict(table=table[:2]), dict(cache=cache[0]),
+                dict(cache=cache.transpose(4, 5)), dict(cache=cache[..., :8]), dict(cache=cache.cpu())):
+        a = dict(table=table, page=8, path=path, count=count, cache=cache)
         a.update(bad)
         with pytest.raises(KernelError):
-            ops.keep_path(cache, batch, a["table"], a["page"], a["path"], a["count"])
+            ops.keep_path(a["cache"], batch, a["table"], a["page"], a["path"], a["count"])
 
 
 # ------------------------------------------------------------------ the controls of logits
@@ -444,3 +445,20 @@ def test_empty_steps(ops):
     ops.keep_path(e(3, 1, 2, 2, 16, 64, device=DEV), batch, i32(np.zeros((0, 4))), 16, i32(np.zeros((0, 4))), none)
     ops.control_logits(e(0, 50, device=DEV), e(0, 50, device=DEV), LogitControls(i32([0]), e(0, 3, device=DEV), none, none, none, none))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tables_without_a_page(ops, dtype):
+    """A table that ends early or has no page in its middle: nothing is read there (keys and values of zeros); the other request is as ever."""
+    c = tree_case(31, dtype, 8, 2, 128, 128, 16, [100, 70], [9, 12])
+    check_tree(run_tree(ops, c, 0.1), c, 0.1)
+    lost = lambda b, lo, hi: [x[b][lo:hi].zero_() for x in (c["keys"], c["values"])]
+    c["table"][0, 2] = -1
+    lost(0, 32, 48)
+    check_tree(run_tree(ops, c, 0.1), c, 0.1)
+    c["table"][1, 0] = c["cache"].shape[0] + 5
+    lost(1, 0, 16)
+    check_tree(run_tree(ops, c, 0.1), c, 0.1)
+    c["table"] = c["table"][:, :5].contiguous()              # request 0 wants seven pages, request 1 six
+    lost(0, 80, 109), lost(1, 80, 82)
+    check_tree(run_tree(ops, c, 0.1), c, 0.1)

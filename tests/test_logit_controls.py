@@ -116,7 +116,7 @@ ONE = 16                                                  # an address that is n
 def test_launchers_refuse_what_they_cannot_take(lib):
     bad, unsupported = -1, -2
     def tree(**kw):
-        a = dict(q=ONE, is_bf16=0, q_start=ONE, pos_start=ONE, parents=ONE, table=ONE, width=4, cache=ONE, layers=1, layer=0, page=16, out=ONE, T=5, B=1, most=5,
+        a = dict(q=ONE, is_bf16=0, q_start=ONE, pos_start=ONE, parents=ONE, table=ONE, width=4, cache=ONE, pages=9, layers=1, layer=0, page=16, out=ONE, T=5, B=1, most=5,
                  nq=4, nkv=2, d=64, dv=64, dc=64, scale=0.1, window=0, softcap=0.0, sink=0, sink_val=None, gate=None, keep=0, splits=1, ws=None, stream=None)
         a.update(kw)
         return lib.tff_attention_tree(*a.values())

@@ -25,7 +25,7 @@ constexpr int BLOCK = 32, JOIN_THREADS = 128, NODE_WORDS = TREE_MAX_NODES / 32;
 
 struct TreeParams {
     const int *q_start, *pos_start, *parents, *block_table;
-    int table_width, layer, nq, nkv, d, dv, window, keep, splits, stages, vec, q_vec;
+    int table_width, pages, layer, nq, nkv, d, dv, window, keep, splits, stages, vec, q_vec;
     float scale, softcap;
     int sink;
     const float *sink_val, *gate;
@@ -102,11 +102,13 @@ attention_tree_kernel(const T* q_in, const T* cache, T* __restrict__ out, const 
     __syncwarp();
 
     // Where key n0 + lane lies: null for keys that no row sees (their slots may hold anything, and their pages may have been given
-    // back), whose stage rows become zeros.  Looked up a block ahead of the copies.
+    // back) and where the table has no page; their stage rows become zeros.  Looked up a block ahead of the copies.
     auto locate = [&](int n0) -> const T* {
         const int n = n0 + lane;
-        if (n > hi || !(n >= lo_tile || n < p.keep)) return nullptr;
-        return cache + (size_t)table[n / p.L.page_size] * p.L.page_stride + (size_t)p.layer * p.L.layer_stride +
+        if (n > hi || !(n >= lo_tile || n < p.keep) || n / p.L.page_size >= p.table_width) return nullptr;
+        const int page = table[n / p.L.page_size];
+        if (page < 0 || page >= p.pages) return nullptr;
+        return cache + (size_t)page * p.L.page_stride + (size_t)p.layer * p.L.layer_stride +
                (size_t)kvh * p.L.head_stride + (size_t)(n % p.L.page_size) * p.L.head_dim;
     };
     auto fetch = [&](const T* at, int stage) {
@@ -365,18 +367,19 @@ TFF_API int tff_attention_tree_splits(int requests, int max_nodes, int max_kv, i
 }
 
 TFF_API int tff_attention_tree(const void* q, int is_bf16, const int* q_start, const int* pos_start, const int* parents,
-                               const int* block_table, int table_width, const void* cache, int cache_layers, int layer, int page_size,
-                               void* out, int num_tokens, int requests, int max_nodes, int nq, int nkv, int d, int dv, int dc,
+                               const int* block_table, int table_width, const void* cache, long long cache_pages, int cache_layers, int layer,
+                               int page_size, void* out, int num_tokens, int requests, int max_nodes, int nq, int nkv, int d, int dv, int dc,
                                float scale, int window, float softcap, int sink, const float* sink_val, const float* gate, int keep,
                                int splits, float* ws, cudaStream_t stream) {
     if (num_tokens <= 0 || requests <= 0 || max_nodes <= 0) return TFF_OK;
     if (!q || !q_start || !pos_start || !parents || !block_table || !cache || !out || nq <= 0 || nkv <= 0 || nq % nkv || d <= 0 ||
-        dv <= 0 || dc < d || dc < dv || page_size <= 0 || softcap < 0.f || keep < 0 || splits < 1 || (splits > 1 && !ws))
+        dv <= 0 || dc < d || dc < dv || page_size <= 0 || cache_pages < 0 || softcap < 0.f || keep < 0 || splits < 1 || (splits > 1 && !ws))
         return TFF_ERR_BAD_ARGUMENT;
     if (d > 512 || dv > 512 || max_nodes > TREE_MAX_NODES || (long long)requests * splits > 65535 || nkv > 65535)
         return TFF_ERR_UNSUPPORTED;
     TreeParams p = {};
     p.q_start = q_start; p.pos_start = pos_start; p.parents = parents; p.block_table = block_table; p.table_width = table_width;
+    p.pages = (int)(cache_pages < 0x7fffffff ? cache_pages : 0x7fffffff);
     p.layer = layer; p.nq = nq; p.nkv = nkv; p.d = d; p.dv = dv;
     p.window = window > 0 ? window : 0; p.keep = window > 0 ? keep : 0;
     p.sink = sink; p.sink_val = sink_val; p.gate = gate; p.scale = scale; p.softcap = softcap; p.splits = splits;

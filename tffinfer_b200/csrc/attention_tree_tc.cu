@@ -52,6 +52,7 @@ struct TreeTcParams {
     int requests, table_width, cache_layers, layer, page_shift, nq, nkv, window, keep, least, extra, whole;
     int group; unsigned group_inverse;               // query heads a kv head, and what a row number is multiplied by for its node
     int tile_rows;                                   // of 128: whole nodes
+    int pages, no_group;                             // of the cache; a group of rows behind its last, which reads as zeros
     float scale_log2, scale_over_cap, cap_log2;
     int sink; const float *sink_val, *gate;
     float *part_o, *part_ml; int4* joins;
@@ -302,14 +303,15 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tm_cache, const __grid_c
                     chunk = first >> 5;
                     ahead = entry(chunk + 1);
                 }
-                const bool valid = lane >= (first & 31) && lane < (first & 31) + ppb && held >= 0;
+                // (a page that the table lacks reads as zeros)
+                const bool valid = lane >= (first & 31) && lane < (first & 31) + ppb && chunk * 32 + lane <= table_end;
                 const unsigned mask = __ballot_sync(0xffffffffu, valid);
                 if (lane == 0) mbar_expect_tx(kv_full(s), (uint32_t)__popc(mask) * (uint32_t)(GROUP << (p.page_shift - 3)));
                 __syncwarp();
                 if (valid) {
                     const long long row = ((((long long)held * p.cache_layers + p.layer) * 2) * p.nkv + piece.kvh) << p.page_shift;
                     tma_load_5d(sKV + s * STAGE_BYTES + (uint32_t)((lane - (first & 31)) * (GROUP << (p.page_shift - 3))), &tm_cache, kv_full(s),
-                                (int)(row >> 3));
+                                (unsigned)held < (unsigned)p.pages ? (int)(row >> 3) : p.no_group);
                 }
                 if (++s == NSTAGES) { s = 0; ++round; }
             }
@@ -785,6 +787,7 @@ TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* 
     p.page_shift = page_size == 8 ? 3 : page_size == 16 ? 4 : page_size == 32 ? 5 : 6;
     p.nq = nq; p.nkv = nkv; p.window = window > 0 ? window : 0; p.keep = window > 0 ? keep : 0;
     p.least = least; p.extra = extra; p.whole = whole;
+    p.pages = (int)(cache_pages < 0x7fffffff ? cache_pages : 0x7fffffff); p.no_group = (int)(rows >> 3);
     p.group = group; p.tile_rows = tile_rows; p.group_inverse = (unsigned)(((1ull << 32) + p.group - 1) / p.group);
     p.scale_log2 = scale * 1.4426950408889634f;
     p.scale_over_cap = softcap > 0.f ? scale / softcap : 0.f;

@@ -15,13 +15,13 @@ constexpr int PER_LANE = MAX_NODES / 32;
 // request: a lane holds the parents and tokens of every 32nd node in registers, so that a step of the walk is a
 // vote a 32 nodes.
 __global__ void __launch_bounds__(32)
-accept_tree_kernel(const int* tokens, const int* parents, const int* drawn, const int* __restrict__ q_start, int num_tokens,
+accept_tree_kernel(const int* tokens, const int* parents, const int* drawn, const int* q_start, int num_tokens,
                    int* __restrict__ path, int* __restrict__ emitted, int* __restrict__ count, int width) {
     __shared__ int draws[MAX_NODES];
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.x, lane = threadIdx.x;
-    const int q0 = q_start[b], n = min(min(q_start[b + 1], num_tokens) - q0, MAX_NODES);
+    const int q0 = __ldcg(q_start + b), n = min(min(__ldcg(q_start + b + 1), num_tokens) - q0, MAX_NODES);
     int up[PER_LANE], word[PER_LANE];
 #pragma unroll
     for (int u = 0; u < PER_LANE; ++u) {
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_path_kernel(const KeepParam
     const int c = (int)(item % row), h = (int)(item / row % p.heads), q = (int)(item / row / p.heads % p.planes);
     const int layer = (int)(item / row / p.heads / p.planes);
     char* base = p.cache + layer * p.layer_bytes + q * p.plane_bytes + h * p.head_bytes + c * (int)sizeof(V);
-    const int pos = p.pos_start[b];
+    const int pos = __ldcg(p.pos_start + b);
     for (int j0 = 1; j0 < n; j0 += AHEAD) {
         if (j0 > 1) __syncthreads();                 // (the slots before have been read)
         if (threadIdx.x < 2 * AHEAD) {
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_path_kernel(const KeepParam
             const long long at = (long long)pos + (threadIdx.x < AHEAD ? i : j);
             long long place = -1;
             if (i != j && i >= 0 && at >= 0 && at / p.page_size < p.table_width) {
-                const int page = p.block_table[(size_t)b * p.table_width + at / p.page_size];
+                const int page = __ldcg(p.block_table + (size_t)b * p.table_width + at / p.page_size);
                 if (page >= 0 && page < p.pages) place = page * p.page_bytes + at % p.page_size * p.row_bytes;
             }
             (threadIdx.x < AHEAD ? from : to)[threadIdx.x % AHEAD] = place;

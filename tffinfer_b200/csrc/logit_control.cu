@@ -25,7 +25,7 @@ namespace {
 constexpr int NT = 256, CTAS_AN_SM = 4;
 constexpr int MAX_NODES = 256;                       // of a request's tree
 constexpr int ROWS_AT_ONCE = 256;
-constexpr int MOST_TOKENS = 12288, LEAST_TOKENS = 1024;        // of a slice: 24 KB of counts beside the rest's 20 leave room for four CTAs an SM
+constexpr int MOST_TOKENS = 17408, LEAST_TOKENS = 1024;        // of a slice: 34 KB of counts beside the rest's 20 leave room for four CTAs an SM
 constexpr int MASK_WORDS = 2304;                     // of masks in shared memory: a part of the rows' at a time
 
 struct ControlParams {
@@ -94,12 +94,12 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
     pdl_wait();
     const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     // (all on their way together)
-    const int r0 = max(0, p.row_start[b]), r1 = min(p.rows, p.row_start[b + 1]);
+    const int r0 = max(0, __ldcg(p.row_start + b)), r1 = min(p.rows, __ldcg(p.row_start + b + 1));
     Penalties penalised;
-    penalised.rep = p.settings[3 * b]; penalised.freq = p.settings[3 * b + 1]; penalised.pres = p.settings[3 * b + 2];
-    const long long first_token = p.history_start[b], held = p.history_len[b];
-    const int prompt = p.prompt_len[b];
-    const int e0 = p.bias_start ? max(0, p.bias_start[b]) : 0, e1 = p.bias_start ? min(p.biases, p.bias_start[b + 1]) : 0;
+    penalised.rep = __ldcg(p.settings + 3 * b); penalised.freq = __ldcg(p.settings + 3 * b + 1); penalised.pres = __ldcg(p.settings + 3 * b + 2);
+    const long long first_token = __ldcg(p.history_start + b), held = __ldcg(p.history_len + b);
+    const int prompt = __ldcg(p.prompt_len + b);
+    const int e0 = p.bias_start ? max(0, __ldcg(p.bias_start + b)) : 0, e1 = p.bias_start ? min(p.biases, __ldcg(p.bias_start + b + 1)) : 0;
     if (r0 >= r1) return;
     penalised.inverse = 1.f / penalised.rep;
     const bool counted = penalised.rep != 1.f || penalised.freq != 0.f || penalised.pres != 0.f;
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
             __syncwarp();
         }
         for (int e = e0 + tid; e < e1; e += NT) {
-            const int t = p.bias_tokens[e];
+            const int t = __ldcg(p.bias_tokens + e);
             if (t >= lo && t < hi) { atomicMin(&bias_range[0], e); atomicMax(&bias_range[1], e + 1); }
         }
         for (int i = tid; i < nodes; i += NT)
@@ -339,10 +339,10 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
             // ascending tokens: equal ones are neighbours, whose values the first of them adds in their order
             for (long long i = tid; i < (long long)(f1 - f0) * n_rows; i += NT) {
                 const int e = f0 + (int)(i / n_rows), r = r0 + (int)(i % n_rows);
-                const int t = p.bias_tokens[e];
-                if (t < lo || t >= hi || (e > e0 && p.bias_tokens[e - 1] == t)) continue;
-                float bias = p.bias_values[e];
-                for (int o = e + 1; o < e1 && p.bias_tokens[o] == t; ++o) bias += p.bias_values[o];
+                const int t = __ldcg(p.bias_tokens + e);
+                if (t < lo || t >= hi || (e > e0 && __ldcg(p.bias_tokens + e - 1) == t)) continue;
+                float bias = __ldcg(p.bias_values + e);
+                for (int o = e + 1; o < e1 && __ldcg(p.bias_tokens + o) == t; ++o) bias += __ldcg(p.bias_values + o);
                 float* to = p.out + (size_t)r * p.vocab + t;
                 *to = bias == -INFINITY ? bias : *to + bias;
             }
@@ -384,6 +384,13 @@ TFF_API int tff_control_logits(const float* logits, float* out, int rows, int vo
     p.slice = slice_tokens(vocab, requests, tff_num_sms());
     const dim3 grid((vocab + p.slice - 1) / p.slice, requests);
     const size_t smem = (size_t)p.slice * 2;
+    static bool configured = false;
+    if (!configured) {
+        if (cudaFuncSetAttribute(control_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_TOKENS * 2) != cudaSuccess ||
+            cudaFuncSetAttribute(control_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_TOKENS * 2) != cudaSuccess)
+            return TFF_ERR_LAUNCH;
+        configured = true;
+    }
     if ((((uintptr_t)logits ^ (uintptr_t)out) & 15) == 0) return tff_launch_pdl(control_kernel<true>, grid, dim3(NT), smem, stream, p);
     return tff_launch_pdl(control_kernel<false>, grid, dim3(NT), smem, stream, p);
 }

@@ -852,7 +852,8 @@ class CudaKernels:
         pos_start[b], its ancestors' and its own.  ``parents`` int32 [T]: an earlier node of the request, or -1 for a node that
         follows the cached tokens.  A node whose chain of parents does not end at -1 (padding: -2) sees nothing, is seen by
         none, and gives zeros.  A node's position, which counts for ``window`` and ``keep``, is pos_start[b] + its
-        ancestors (the queries and keys are rotated by it: ``batch.positions`` of such a step).  At most 256 nodes a request."""
+        ancestors (the queries and keys are rotated by it: ``batch.positions`` of such a step).  At most 256 nodes a request.
+        The keys and values of cached tokens and of nodes that are there are finite; padding's may be anything."""
         T, B, dtype = q.shape[0], batch.num_requests, q.dtype
         dc = kv_cache.shape[-1]
         self._need_here(dtype, (q, out))
@@ -908,7 +909,7 @@ class CudaKernels:
     def _attention_tree_plain(self, q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window,
                               softcap, sink, gates, keep, splits=None) -> None:
         T, B = q.shape[0], batch.num_requests
-        c_ptr, _, c_layers, c_layer = self._cache_args(kv_cache, kv_layer)
+        c_ptr, c_pages, c_layers, c_layer = self._cache_args(kv_cache, kv_layer)
         sink_on, sink_val = self._sink_args(sink, nq)
         if splits is None:
             graph = getattr(batch, "graph_bucket", None) is not None
@@ -918,8 +919,8 @@ class CudaKernels:
         ws = torch.empty(T * nq * splits * (dv + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
         self._check(self.lib.tff_attention_tree(
             _ptr(q), _c_int(_dt(q)), _ptr(batch.q_start), _ptr(batch.pos_start), _ptr(parents), _ptr(block_table),
-            _c_int(block_table.shape[1]), c_ptr, _c_int(c_layers), _c_int(c_layer), _c_int(page_size), _ptr(out), _c_int(T), _c_int(B),
-            _c_int(batch.max_q_len), _c_int(nq), _c_int(nkv), _c_int(d), _c_int(dv), _c_int(kv_cache.shape[-1]), _c_float(scale),
+            _c_int(block_table.shape[1]), c_ptr, _c_int(c_pages), _c_int(c_layers), _c_int(c_layer), _c_int(page_size), _ptr(out), _c_int(T),
+            _c_int(B), _c_int(batch.max_q_len), _c_int(nq), _c_int(nkv), _c_int(d), _c_int(dv), _c_int(kv_cache.shape[-1]), _c_float(scale),
             _c_int(window), _c_float(softcap), _c_int(1 if sink_on else 0), _ptr(sink_val), _ptr(gates), _c_int(keep), _c_int(splits),
             _ptr(ws), self._stream()), "attention_tree")
         self.launches += 2 if splits > 1 else 1
@@ -950,8 +951,11 @@ class CudaKernels:
         path and count as ``accept_tree`` gives them (a path's nodes ascend); the slots behind stay as they are."""
         B = batch.num_requests
         self._need_here(_I32, (block_table, path, count, batch.pos_start))
-        if kv_cache.dim() != 6 or kv_cache.shape[4] != page_size:
+        if kv_cache.dim() != 6:
             raise KernelError("the cache is [pages, layers, planes, kv heads, page, head]")
+        (pages, layers, planes, heads, page, d), strides = kv_cache.shape, kv_cache.stride()
+        if page != page_size or strides[2:] != (heads * page * d, page * d, d, 1):
+            raise KernelError(f"a page of the cache is dense and holds {page_size} slots")
         if kv_cache.get_device() != path.get_device():
             raise KernelError("the cache is on another device")
         if path.dim() != 2 or path.shape[0] != B or count.numel() != B or block_table.dim() != 2 or block_table.shape[0] < B or \
@@ -959,11 +963,9 @@ class CudaKernels:
             raise KernelError("paths [requests, width], a count and a row of the block table a request")
         if B == 0 or path.shape[1] <= 1 or kv_cache.numel() == 0:
             return
-        self._cache_args(kv_cache, 0)                          # (refuses what is neither form of a cache)
-        pages, layers, planes, heads, _, d = kv_cache.shape
         size = kv_cache.element_size()
         self._check(self.lib.tff_keep_path(_ptr(kv_cache), _c_int(pages), _c_int(layers), _c_int(planes), _c_int(heads), _c_int(page_size),
-                                           _c_int(d * size), _c_int(kv_cache.stride(0) * size), _c_int(kv_cache.stride(1) * size),
+                                           _c_int(d * size), _c_int(strides[0] * size), _c_int(strides[1] * size),
                                            _ptr(batch.pos_start), _ptr(block_table), _c_int(block_table.shape[1]), _ptr(path),
                                            _ptr(count), _c_int(B), _c_int(path.shape[1]), self._stream()), "keep_path")
         self.launches += 1
