@@ -103,6 +103,23 @@ def test_the_sampler_controls_the_rows_whose_requests_ask_for_it():
     assert ops.calls == ["repetition_penalty"]           # a repetition penalty alone goes the way it went
 
 
+def test_draws_that_lack_what_their_controls_need():
+    s, logits = Sampler(_PlainOps(), "cpu"), torch.zeros(1, 4)
+    for p in (SamplingParams(frequency_penalty=0.1), SamplingParams(presence_penalty=0.1), SamplingParams(token_mask=lambda made: None)):
+        with pytest.raises(ValueError, match="needs the requests' tokens"):
+            s.sample(logits, [p], [0], [0])
+        with pytest.raises(ValueError, match="needs the requests' tokens"):
+            s.sample(logits, [p], [0], [0], [[1]])
+    s.sample(logits, [SamplingParams(logit_bias=((1, 1.0),))], [0], [0])      # a bias needs none
+
+
+def test_options_that_float32_and_int32_do_not_hold():
+    for kw in (dict(frequency_penalty=1e39), dict(presence_penalty=-1e39), dict(logit_bias=((0, 1e39),)), dict(logit_bias=((2**31, 1.0),)),
+               dict(frequency_penalty=math.nan)):
+        with pytest.raises(ValueError):
+            SamplingParams(**kw)
+
+
 @pytest.fixture(scope="module")
 def lib():
     lib = ctypes.CDLL(build.library_path(build=True, verbose=False))

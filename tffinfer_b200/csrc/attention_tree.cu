@@ -13,6 +13,10 @@
 // 32, which come to shared memory once for all its rows; a warp has up to 4 rows: for the scores a lane is a key, for the values a
 // lane has 4 (8, 16) columns.  What a row sees of a block is a word with a bit a key.  The shares' results (maximum, sum, weighted
 // values) are joined by a second kernel.
+//
+// What bounds it: shared-memory reads (every warp reads the whole block) and, in small steps, chains of them: two trees of 13 nodes behind 550
+// tokens (16/8 heads of 128, float32) 23 us; with 8 warps of four rows 28, and 43 with a reference that moves and a sum that is added across
+// the warp with every block.
 #include "common.cuh"
 #include "attention_common.h"
 #include "attention_tree.cuh"

@@ -17,7 +17,18 @@
 // tokens' last are masked: a row builds a word of 64 bits from its chain of parents, which lie in shared memory.
 //   warps 0-7     softmax, rescale, outputs of the first tile (tensor memory lanes 32 * (warp % 4) ..)
 //   warps 8-15    the same for the second tile (QT = 2)
-//   then          TMA producer: one box a page into a ring of stages, without a pause between pieces; an issuing warp a tile
+//   then          TMA producer: one box a page into a ring of stages, without a pause between pieces; an issuing warp a tile, which
+//                 asks for the queries of the next piece as soon as the products have read the last one's
+// What bounds it (cycles counted in the kernel on a B200, heads of 128): with one tile a CTA a block of keys and values, 32 KB, takes 1,150
+// cycles, about what the memory gives an SM: 64 trees of 8 nodes behind 200 to 6,000 tokens (32/8 heads) 148 us, 5.4 TB/s.  With two tiles it takes
+// 1,590, the products' and exponentials' time: a tree of 64 nodes behind 32,000 tokens (64/8 heads) 83 to 95 us by the clock
+// that the power cap leaves.  Around that, a CTA's first scores come 7,500 to 10,000 cycles after its start (2,900 for its place in the line, 3,500 for the
+// first keys), and a second piece costs about six blocks: 8 trees of 32 nodes behind 2,048 tokens 26.5 us, 71 MB.
+//   - The queries go ahead of all but two blocks of keys: behind a full ring of every CTA's they came 7,000 cycles later.
+//   - A walk counts ``extra`` = 6 units more than its blocks: 3 gives 94.4 / 27.8 us (the long tree / the 8 trees), 5 and 7 92.3, 91.2 / 27.2, 27.3, and
+//     12 91.2 / 28.7.
+//   - A share has at least ``least`` = 4 units: one request of 32/8 heads behind 800 tokens 11.8 us, with 1 14.3, with 12 16.1; behind 2,048 14.9, 16.8, 16.3.
+//   - Short walks are not divided (CudaKernels.TREE_WHOLE_BLOCKS).
 // Every mbarrier wait is bounded; a timeout raises the library's error word.
 #define TFF_SUSPENDED_WAITS
 #include "tcgen05.cuh"
@@ -753,13 +764,13 @@ int launch(const CUtensorMap& tm, const CUtensorMap& tq, const TreeTcParams& p, 
 }  // namespace
 
 // TFF_ERR_UNSUPPORTED, with nothing launched, for what the general kernel (attention_tree.cu) has to take.  A CTA's share has at least
-// ``least`` units, a walk ``extra`` of them ahead of its blocks; ``whole``: no walk is divided, and there is no second kernel.  ``ws``: an SM has 4 words and room for two pieces of 128 rows (256 where some request may have more rows
-// than 128) of d + 2 floats.
+// ``least`` units, a walk ``extra`` of them ahead of its blocks; ``whole``: no walk is divided, and there is no second kernel.  ``ws``: an
+// SM has 4 words and room for two pieces of 128 rows (256 where some request may have more rows than a tile) of d + 2 floats.
 TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* pos_start, const int* parents, const int* block_table,
                                   int table_width, const void* cache, long long cache_pages, int cache_layers, int layer, int page_size,
                                   void* out, int num_tokens, int requests, int max_nodes, int nq, int nkv, int d, float scale, int window,
                                   float softcap, int sink, const float* sink_val, const float* gate, int keep, int least, int extra, int whole, void* ws,
-                                  long long ws_floats, cudaStream_t stream) {
+                                  long long ws_floats, cudaStream_t stream) try {
     if (num_tokens <= 0 || requests <= 0 || max_nodes <= 0) return TFF_OK;
     if (!q || !q_start || !pos_start || !parents || !block_table || !cache || !out || nq <= 0 || nkv <= 0 || nq % nkv || softcap < 0.f ||
         keep < 0 || least <= 0 || extra < 0 || extra > 64 || table_width <= 0 || (!whole && !ws))
@@ -798,6 +809,9 @@ TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* 
     p.part_ml = p.part_o + (size_t)sms * 2 * qt * BLOCK_M * d;
     p.error_flag = tff_device_error_flag();
     if (p.error_flag == nullptr) return TFF_ERR_LAUNCH;
-    if (d == 128) return qt == 2 ? launch<128, 2>(tm, tq, p, sms, qt == 2 ? 2 * BLOCK_M : max_nodes * group, stream) : launch<128, 1>(tm, tq, p, sms, qt == 2 ? 2 * BLOCK_M : max_nodes * group, stream);
-    return qt == 2 ? launch<64, 2>(tm, tq, p, sms, qt == 2 ? 2 * BLOCK_M : max_nodes * group, stream) : launch<64, 1>(tm, tq, p, sms, qt == 2 ? 2 * BLOCK_M : max_nodes * group, stream);
+    const int rows_at_most = qt == 2 ? 2 * BLOCK_M : max_nodes * group;
+    if (d == 128) return qt == 2 ? launch<128, 2>(tm, tq, p, sms, rows_at_most, stream) : launch<128, 1>(tm, tq, p, sms, rows_at_most, stream);
+    return qt == 2 ? launch<64, 2>(tm, tq, p, sms, rows_at_most, stream) : launch<64, 1>(tm, tq, p, sms, rows_at_most, stream);
+} catch (...) {                                                  // (the tensor maps' tables: no memory for another)
+    return TFF_ERR_DRIVER;
 }

@@ -3,6 +3,10 @@
 //
 // Node i of request b is row q_start[b] + i of the step and has cache slot pos_start[b] + i; its parent is an earlier node,
 // node 0 (the token drawn last, parent -1) the root.
+//
+// Measured in a captured run: the walk 1.7 us for one tree of 8 nodes, 2.6 for 64 of 64 (a launch and two trips to memory; 11 to 16
+// votes of the warp are a fraction of that); the move 2.4 us for one path in 8 layers, 18.9 for 64 paths in 36 layers of 8 heads of 128 (60 MB
+// read and written, 3.2 TB/s), 25 with four loads ahead and the places looked up by every thread.
 #include "common.cuh"
 
 namespace {

@@ -831,7 +831,10 @@ class CudaKernels:
                                        softcap, sink, gates, keep)
 
     TREE_MAX_NODES = 256          # of a request's tree of drafted tokens
-    TREE_WHOLE_BLOCKS = 12        # up to so many blocks of 64 keys a request's walk is not divided
+    # Up to so many blocks of 64 keys a request's walk is not divided: 8 requests behind 500 tokens (32/8 heads) 11.4 us instead of 13.4, 32
+    # behind 600 (64/8) 29 instead of 33, one behind 500 10.9 instead of 10.7, and a launch less in all (the host's time of a call 18
+    # instead of 21); at 13 and more, one behind 800 13.9 instead of 11.8, 4 behind 1,000 (16/8) 17.4 instead of 15.2.
+    TREE_WHOLE_BLOCKS = 12
 
     def _tree_args(self, batch, parents, T: int) -> None:
         """Checks the sizes of what the kernels of drafted trees are given of a step."""
@@ -867,6 +870,8 @@ class CudaKernels:
             self._need_here(_F32, (gates,))
             if gates.shape != (T, nq):
                 raise KernelError("head gates are [T, nq]")
+        if isinstance(sink, torch.Tensor):
+            self._need_here(_F32, (sink,))
         if block_table.dim() != 2 or block_table.shape[0] < B:
             raise KernelError("the block table is [requests, pages]")
         if not 0 <= kv_layer < kv_cache.shape[1]:
@@ -883,7 +888,8 @@ class CudaKernels:
     def _attention_tree_tc(self, q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, scale, window,
                            softcap, sink, gates, keep, least: int = 4, extra: int = 6, whole=None) -> bool:
         """On the tensor cores; False, and nothing launched, for what that kernel does not take.  ``least``: blocks of 64 keys that
-        a CTA's share has at least; ``extra``: how many of them a piece of a walk costs beside its own; ``whole``: shares are whole walks (None: where none has more than WHOLE_BLOCKS)."""
+        a CTA's share has at least; ``extra``: how many of them a piece of a walk costs beside its own; ``whole``: shares
+        are whole walks (None: where none has more than TREE_WHOLE_BLOCKS)."""
         T, B = q.shape[0], batch.num_requests
         if whole is None:
             keys = block_table.shape[1] * page_size if getattr(batch, "graph_bucket", None) is not None else int(batch.max_kv_len)

@@ -19,6 +19,9 @@ TOP_P = "top_p"
 STRATEGIES = ("default", GREEDY, RANDOM, TOP_K, TOP_P)   # FOR_EACH_STRATEGY, LLMSampler.h:18-24
 
 
+_FLOAT32_MAX = float(np.finfo(np.float32).max)
+
+
 @dataclass(frozen=True)
 class SamplingParams:
     type: str = GREEDY                 # "greedy": temperature and filters are ignored
@@ -34,7 +37,7 @@ class SamplingParams:
     presence_penalty: float = 0.0      # taken off a token's logit once it was generated
     logit_bias: Tuple[Tuple[int, float], ...] = ()        # (token, what is added to its logit; -infinity bans it)
     # a grammar: the generated tokens so far -> 32-bit words with a bit for every allowed token (token t: bit t % 32 of word
-    # t // 32), or None for no limit
+    # t // 32), or None for no limit.  At least one token is allowed; it does not raise (the step that asks has run by then)
     token_mask: Optional[Callable[[List[int]], Optional[np.ndarray]]] = None
 
     def __post_init__(self):
@@ -46,10 +49,10 @@ class SamplingParams:
             raise ValueError("top_k >= 0, 0 < top_p <= 1 and 0 <= min_p < 1 are required")
         if self.repetition_penalty <= 0:
             raise ValueError("repetition_penalty must be > 0")
-        if not (math.isfinite(self.frequency_penalty) and math.isfinite(self.presence_penalty)):
-            raise ValueError("frequency_penalty and presence_penalty must be finite")
-        if any(t < 0 or not v < math.inf for t, v in self.logit_bias):
-            raise ValueError("logit_bias is pairs of a token id and a finite number or -infinity")
+        if not (abs(self.frequency_penalty) <= _FLOAT32_MAX and abs(self.presence_penalty) <= _FLOAT32_MAX):
+            raise ValueError("frequency_penalty and presence_penalty must be finite in float32")
+        if any(not 0 <= t < 2**31 or not v <= _FLOAT32_MAX for t, v in self.logit_bias):
+            raise ValueError("logit_bias is pairs of a token id and a number that is finite in float32, or -infinity")
         if self.max_new_tokens < 0:
             raise ValueError("max_new_tokens must be >= 0")
 
