@@ -462,3 +462,33 @@ def test_tables_without_a_page(ops, dtype):
     c["table"] = c["table"][:, :5].contiguous()              # request 0 wants seven pages, request 1 six
     lost(0, 80, 109), lost(1, 80, 82)
     check_tree(run_tree(ops, c, 0.1), c, 0.1)
+
+
+def test_banned_tokens_are_never_drawn(ops):
+    # Every second token is banned, and the numbers that are drawn with lie at the ends of the allowed tokens' stretches, within a
+    # few roundings: whichever way those fall, the draw is an allowed token.
+    V, near = 2048, 8
+    x = torch.randn(V, generator=torch.Generator().manual_seed(3)) * 2
+    bits = np.zeros(V, dtype=bool)
+    bits[::2] = True
+    mask = torch.from_numpy(np.packbits(bits, bitorder="little").view(np.int32).copy()).view(1, -1)
+    ends = torch.cumsum(torch.exp(x[::2].double()), 0)
+    u = (ends / ends[-1]).float().repeat_interleave(near)
+    u = (u + (torch.arange(u.numel()) % near - near // 2) * u * 2.0**-24).clamp(0.0, 1.0 - 2.0**-24)
+    R = u.numel()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    controls = LogitControls(i32([0, R]), torch.tensor([[1.0, 0.0, 0.0]], device="cuda"), i32([]), i32([0]), i32([0]), i32([0]), mask=mask.cuda(),
+                             mask_row=torch.zeros(R, dtype=torch.int32, device="cuda"))
+    logits = x.cuda().repeat(R, 1)
+    ops.control_logits(logits, logits, controls)
+    out = torch.empty(R, dtype=torch.int32, device="cuda")
+    one = torch.ones(R, device="cuda")
+    for filters in ({}, dict(top_k=i32([700] * R), top_p=one * 0.999, min_p=one * 0)):
+        ops.sample(logits, one, u.cuda(), out, **filters)
+        assert not (out % 2).any()
+    # a row whose mask leaves nothing gives some token of the vocabulary
+    logits.fill_(-math.inf)
+    for filters in ({}, dict(top_k=i32([700] * R), top_p=one * 0.999, min_p=one * 0)):
+        ops.sample(logits, one, u.cuda(), out, **filters)
+        assert ((out >= 0) & (out < V)).all()
+    ops.check_errors()

@@ -286,7 +286,7 @@ sample_kernel(const float* __restrict__ logits, const float* __restrict__ temper
         int pick = -1, last = -1;
         for (int i = lo; i < hi; ++i) {
             const float z = (row[i] - mx) * invT;
-            if (z < cut) continue;
+            if (z < cut || z == -INFINITY) continue;      // (a banned token is not drawn, whichever way the sums are rounded)
             last = i;
             c += expf(z);
             if (target < c) { pick = i; break; }
