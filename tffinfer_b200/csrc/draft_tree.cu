@@ -5,8 +5,9 @@
 // node 0 (the token drawn last, parent -1) the root.
 //
 // Measured in a captured run: the walk 1.7 us for one tree of 8 nodes, 2.6 for 64 of 64 (a launch and two trips to memory; 11 to 16
-// votes of the warp are a fraction of that); the move 2.4 us for one path in 8 layers, 18.9 for 64 paths in 36 layers of 8 heads of 128 (60 MB
-// read and written, 3.2 TB/s), 25 with four loads ahead and the places looked up by every thread.
+// votes of the warp are a fraction of that); the move 2.4 us for one path in 8 layers, 15.4 for 64 paths in 36 layers of 8 heads of 128 (60 MB
+// read and written, 3.9 TB/s); 18.9 with the places divided in 64 bits, 25 with four loads ahead and the places looked up by every
+// thread, 15.6 to 16.4 with two or three items a thread.
 #include "common.cuh"
 
 namespace {
@@ -60,8 +61,8 @@ constexpr int KEEP_THREADS = 256, AHEAD = 8;
 
 struct KeepParams {
     char* cache; long long page_bytes, layer_bytes, plane_bytes, head_bytes;
-    int pages, layers, planes, heads, page_size, row_bytes;
-    const int *pos_start, *block_table; int table_width;
+    int pages; unsigned layers, planes, heads, page_size, row_bytes;
+    const int *pos_start, *block_table; unsigned table_width;
     const int *path, *count; int width;
 };
 
@@ -76,27 +77,27 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_path_kernel(const KeepParam
     const int b = blockIdx.y;
     const int n = min(__ldcg(p.count + b), p.width);
     if (n <= 1) return;
-    const int row = p.row_bytes / (int)sizeof(V);
-    const long long item = (long long)blockIdx.x * KEEP_THREADS + threadIdx.x;
-    const bool mine = item < (long long)p.layers * p.planes * p.heads * row;
-    const int c = (int)(item % row), h = (int)(item / row % p.heads), q = (int)(item / row / p.heads % p.planes);
-    const int layer = (int)(item / row / p.heads / p.planes);
-    char* base = p.cache + layer * p.layer_bytes + q * p.plane_bytes + h * p.head_bytes + c * (int)sizeof(V);
+    const unsigned row = p.row_bytes / (unsigned)sizeof(V);
+    const unsigned item = blockIdx.x * KEEP_THREADS + threadIdx.x;
+    const unsigned r = item / row, plane = r / p.heads, layer = plane / p.planes;
+    char* base = p.cache + layer * p.layer_bytes + (plane - layer * p.planes) * p.plane_bytes + (r - plane * p.heads) * p.head_bytes +
+                 (item - r * row) * (unsigned)sizeof(V);
     const int pos = __ldcg(p.pos_start + b);
     for (int j0 = 1; j0 < n; j0 += AHEAD) {
         if (j0 > 1) __syncthreads();                 // (the slots before have been read)
         if (threadIdx.x < 2 * AHEAD) {
             const int j = j0 + threadIdx.x % AHEAD, i = j < n ? __ldcg(p.path + (size_t)b * p.width + j) : j;
             const long long at = (long long)pos + (threadIdx.x < AHEAD ? i : j);
+            const unsigned entry = (unsigned)at / p.page_size;           // (at least 0, and below 2^32)
             long long place = -1;
-            if (i != j && i >= 0 && at >= 0 && at / p.page_size < p.table_width) {
-                const int page = __ldcg(p.block_table + (size_t)b * p.table_width + at / p.page_size);
-                if (page >= 0 && page < p.pages) place = page * p.page_bytes + at % p.page_size * p.row_bytes;
+            if (i != j && i >= 0 && at >= 0 && entry < p.table_width) {
+                const int page = __ldcg(p.block_table + (size_t)b * p.table_width + entry);
+                if (page >= 0 && page < p.pages) place = page * p.page_bytes + (long long)((unsigned)at - entry * p.page_size) * p.row_bytes;
             }
             (threadIdx.x < AHEAD ? from : to)[threadIdx.x % AHEAD] = place;
         }
         __syncthreads();
-        if (!mine) continue;
+        if (layer >= p.layers) continue;
         V v[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
@@ -136,7 +137,7 @@ TFF_API int tff_keep_path(void* cache, int pages, int layers, int planes, int he
     const int v = align % 16 == 0 ? 16 : align % 4 == 0 ? 4 : 2;
     const long long items = (long long)layers * planes * heads * (row_bytes / v);
     const long long blocks = (items + KEEP_THREADS - 1) / KEEP_THREADS;
-    if (blocks > 0x7fffffff) return TFF_ERR_UNSUPPORTED;
+    if (items > 0x7fffffff) return TFF_ERR_UNSUPPORTED;           // (counted in 32 bits)
     const dim3 grid((unsigned)blocks, requests);
     if (v == 16) return tff_launch_pdl(keep_path_kernel<uint4>, grid, dim3(KEEP_THREADS), (size_t)0, stream, p);
     if (v == 4) return tff_launch_pdl(keep_path_kernel<unsigned>, grid, dim3(KEEP_THREADS), (size_t)0, stream, p);
