@@ -11,12 +11,17 @@
 //
 // A CTA takes a slice of the vocabulary for all rows of one request: it counts the history's tokens of its slice in shared
 // memory (integers: in any order), once for all rows, and then streams the rows' slices, four logits a load and four loads a
-// thread on their way, of four rows where there are as many.  What bounds it beside the traffic is instructions: a thread's
-// addresses are a pointer and an offset, and what a count does to a logit is worked out once for four rows, and not at all where none of a
-// thread's four tokens was seen (looked up and divided for every logit, 140 to 230 instructions for a warp's 128 of them, 256 rows of
-// trees took 62 us and 64 rows 30).  The few tokens of a row's path and the few biased ones are put right behind that pass.  Where a
-// mask allows none of a load's four tokens nothing is read.  Tried without gain: counted tokens put right behind a pass that only copies
-// (98 us and 34), parts of rows by bulk copies through shared memory (75 and 41: half the instructions, too few warps).
+// thread on their way, of four rows where there are as many.  The few tokens of a row's path and the few biased ones are put right
+// behind that pass.  Where a mask allows none of a load's four tokens nothing is read.
+//
+// What bounds it beside the traffic: instructions, and the warps that hide the way to memory.  A thread's addresses are a pointer and
+// an offset, and what a count does to a logit is worked out once for four rows, and not at all where none of a thread's four tokens was
+// seen (looked up and divided for every logit, 140 to 230 instructions for a warp's 128 of them, 256 rows of trees took 62 us and 64
+// rows 30).  Measured at a vocabulary of 151,936 with masks and 200 to 6,000 tokens of history: 64 rows 26.5 to 28 us (78 MB, 2.9
+// TB/s; a plain pass over as many bytes 13.4), the 256 nodes of eight trees 57 (5.4 TB/s; 47), one row without a mask 4.6 to 5.5.
+//   Four CTAs an SM; with three, and larger slices, 29 and 62.  Tried without gain (64 rows, 256 nodes): the next loads ahead of a
+//   thread's work, 32 and 71 (registers for three CTAs an SM); a branch for each of a thread's tokens, 28 and 58; counted tokens put right behind a
+//   pass that only copies, 34 and 98; parts of rows by bulk copies through shared memory, 41 and 75 (half the instructions, too few warps).
 #include "common.cuh"
 #include "tma_host.h"
 
