@@ -362,9 +362,10 @@ TFF_API int tff_attention_tree_splits(int requests, int max_nodes, int max_kv, i
     const long long ctas = (rows + tile - 1) / tile * nkv * requests;
     long long keys = max_kv;
     if (window > 0 && (long long)window + keep + max_nodes < keys) keys = (long long)window + keep + max_nodes;
-    // a CTA an SM where that makes four shares or more (of 16 warps then: dispatch), else two
+    // A CTA an SM where that makes four shares or more of 32 rows (of 16 warps then: dispatch), else two; for smaller tiles two where their
+    // stages leave room for both (one request of 8 nodes behind 4,000 tokens, 16/8 heads: 31 us, with one 40; of 4 behind 16,000, 8/8: 56 and 85)
     long long s = sms / ctas;
-    if (s < 4) s = 2ll * sms / ctas;
+    if (s < 4 || (tile < 32 && dv <= 128)) s = 2ll * sms / ctas;
     if (s > keys / (2 * BLOCK)) s = keys / (2 * BLOCK);
     if (s > 32) s = 32;
     return s < 1 || requests * s > 65535 ? 1 : (int)s;
