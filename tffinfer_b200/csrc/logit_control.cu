@@ -17,8 +17,9 @@
 // What bounds it beside the traffic: instructions, and the warps that hide the way to memory.  A thread's addresses are a pointer and
 // an offset, and what a count does to a logit is worked out once for four rows, and not at all where none of a thread's four tokens was
 // seen (looked up and divided for every logit, 140 to 230 instructions for a warp's 128 of them, 256 rows of trees took 62 us and 64
-// rows 30).  Measured at a vocabulary of 151,936 with masks and 200 to 6,000 tokens of history: 64 rows 26.5 to 28 us (78 MB, 2.9
-// TB/s; a plain pass over as many bytes 13.4), the 256 nodes of eight trees 57 (5.4 TB/s; 47), one row without a mask 4.6 to 5.5.
+// rows 30).  Measured at a vocabulary of 151,936 with masks and 200 to 6,000 tokens of history: 64 rows 24.8 us (78 MB, 3.1
+// TB/s; a plain pass over as many bytes 13.4: the rest is what comes ahead of the first logits, 11,000 cycles of loads that wait for
+// one another), the 256 nodes of eight trees 56 (5.5 TB/s; 47), one row without a mask 5.2.
 //   Four CTAs an SM; with three, and larger slices, 29 and 62.  Tried without gain (64 rows, 256 nodes): the next loads ahead of a
 //   thread's work, 32 and 71 (registers for three CTAs an SM); a branch for each of a thread's tokens, 28 and 58; counted tokens put right behind a
 //   pass that only copies, 34 and 98; parts of rows by bulk copies through shared memory, 41 and 75 (half the instructions, too few warps).
@@ -140,22 +141,57 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
         const int most = p.mask ? min(ROWS_AT_ONCE, MASK_WORDS / words) : ROWS_AT_ONCE, parts = (r1 - r0 + most - 1) / most;
         const int at_once = min(most, ((r1 - r0 + parts - 1) / parts + 3) & ~3);
         __syncthreads();                             // (the part before is through with the counts)
-        if (len > 0) for (int i = tid; i < p.slice / 8; i += NT) reinterpret_cast<uint4*>(count_words)[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (tid == 0) { hit_count = 0; bias_range[0] = e1; bias_range[1] = e0; }
-        __syncthreads();
-        // Four tokens a load, from the 16 bytes on in which the history begins.  Few of them are the slice's: a warp lists those of its
-        // 512 tokens and then counts them a lane each.  (With a branch for every token nearly every one was taken by some lane.)
+        // The first history tokens, the masks of the first rows and the counts' zeros are on their way together.
         const int* at = p.history + first_token;
         const int skew = (int)((uintptr_t)at >> 2 & 3), warp0 = tid & ~31;
-        unsigned short* list = lists[tid >> 5];
-        for (int g0 = 0; (g0 + warp0) * 4 - skew < len; g0 += 4 * NT) {
-            int4 t4[4];
+        int4 t4[4];
+        auto tokens_of = [&](int g0) {               // four tokens a load, from the 16 bytes on in which the history begins
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int g = g0 + u * NT + tid;
                 t4[u] = make_int4(-1, -1, -1, -1);
                 if (g * 4 - skew < len) t4[u] = __ldcg(reinterpret_cast<const int4*>(at - skew) + g);
             }
+        };
+        tokens_of(0);
+        // A single row is asked for while the history is counted, 32 tokens of a mask's word at a time (64 rows 26.3 -> 24.9 us; rows of trees
+        // come to warps that have others to wait for: 256 of them 56 us, and 63 with this).
+        const bool single = r1 - r0 == 1;
+        auto ahead = [&](int word) {
+            const int t = max(lo, (w0 + word) * 32);
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(p.logits + (size_t)r0 * p.vocab + t));
+        };
+        if (single && !p.mask) for (int i = tid; i < words; i += NT) ahead(i);
+        int biased = e0 + tid < e1 ? __ldcg(p.bias_tokens + e0 + tid) : -1;
+        bool masked = false;
+        auto masks_of = [&](int c0, int rows) {      // which of rows c0 .. have one
+            masked = false;
+            for (int i = tid; i < rows; i += NT) { mask_at[i] = mask_of(c0 + i); masked = masked || mask_at[i] >= 0; }
+        };
+        auto mask_words_of = [&](int rows) {
+            for (int i = tid; i < rows * words; i += NT) {
+                const int m = mask_at[i / words];
+                const unsigned word = m < 0 ? 0xffffffffu : __ldcg(p.mask + (size_t)m * p.mask_words + w0 + i % words);
+                masks[i] = word;
+                if (single && word) ahead(i);
+            }
+        };
+        if (p.mask) masks_of(r0, min(at_once, r1 - r0));
+        if (len > 0) for (int i = tid; i < p.slice / 8; i += NT) reinterpret_cast<uint4*>(count_words)[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (tid == 0) { hit_count = 0; bias_range[0] = e1; bias_range[1] = e0; }
+        masked = __syncthreads_or(masked);
+        for (int e = e0 + tid; e < e1; e += NT) {
+            if (biased >= lo && biased < hi) { atomicMin(&bias_range[0], e); atomicMax(&bias_range[1], e + 1); }
+            biased = e + NT < e1 ? __ldcg(p.bias_tokens + e + NT) : -1;
+        }
+        for (int i = tid; i < nodes; i += NT)
+            if (token[i] >= lo && token[i] < hi) hits[atomicAdd(&hit_count, 1)] = (short)i;
+        if (masked) mask_words_of(min(at_once, r1 - r0));
+        // Few tokens are the slice's: a warp lists those of its 512 and then counts them a lane each.  (With a branch for every token
+        // nearly every one was taken by some lane.)
+        unsigned short* list = lists[tid >> 5];
+        for (int g0 = 0; (g0 + warp0) * 4 - skew < len; g0 += 4 * NT) {
+            if (g0 > 0) tokens_of(g0);
             int n = 0;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -174,30 +210,20 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
             for (int i = lane; i < n; i += 32) counts.add(list[i] & 0x7fff, list[i] >> 15);
             __syncwarp();
         }
-        for (int e = e0 + tid; e < e1; e += NT) {
-            const int t = __ldcg(p.bias_tokens + e);
-            if (t >= lo && t < hi) { atomicMin(&bias_range[0], e); atomicMax(&bias_range[1], e + 1); }
-        }
-        for (int i = tid; i < nodes; i += NT)
-            if (token[i] >= lo && token[i] < hi) hits[atomicAdd(&hit_count, 1)] = (short)i;
 
         // ------------------------------------------------ the rows' slices
         for (int c0 = r0; c0 < r1; c0 += at_once) {
             const int rows = min(at_once, r1 - c0);
-            bool masked = false;
-            if (p.mask) {
-                if (c0 > r0) __syncthreads();
-                for (int i = tid; i < rows; i += NT) { mask_at[i] = mask_of(c0 + i); masked = masked || mask_at[i] >= 0; }
+            if (c0 == r0) {
+                __syncthreads();                     // the counts and the first rows' masks are there
+            } else if (p.mask) {
+                __syncthreads();
+                masks_of(c0, rows);
                 masked = __syncthreads_or(masked);
                 if (masked) {
-                    for (int i = tid; i < rows * words; i += NT) {
-                        const int m = mask_at[i / words];
-                        masks[i] = m < 0 ? 0xffffffffu : __ldcg(p.mask + (size_t)m * p.mask_words + w0 + i % words);
-                    }
+                    mask_words_of(rows);
                     __syncthreads();
                 }
-            } else if (c0 == r0) {
-                __syncthreads();
             }
             auto one = [&](int row, int t) {
                 const size_t i = (size_t)(c0 + row) * p.vocab + t;
