@@ -5,9 +5,9 @@
 // node 0 (the token drawn last, parent -1) the root.
 //
 // Measured in a captured run: the walk 1.7 us for one tree of 8 nodes, 2.6 for 64 of 64 (a launch and two trips to memory; 11 to 16
-// votes of the warp are a fraction of that); the move 2.4 us for one path in 8 layers, 15.4 for 64 paths in 36 layers of 8 heads of 128 (60 MB
-// read and written, 3.9 TB/s); 18.9 with the places divided in 64 bits, 25 with four loads ahead and the places looked up by every
-// thread, 15.6 to 16.4 with two or three items a thread.
+// votes of the warp are a fraction of that); the move 1.9 us for one path in 8 layers, 14.6 for 64 paths in 36 layers of 8 heads of 128 (60 MB
+// read and written, 4.1 TB/s).  Registers for four CTAs an SM count: 16.9 with 80 of them; 18.9 with the places divided in 64 bits, 25 with
+// four loads ahead and the places looked up by every thread, 16.4 with two items a thread.
 #include "common.cuh"
 
 namespace {
@@ -72,21 +72,29 @@ struct KeepParams {
 template <typename V>
 __global__ void __launch_bounds__(KEEP_THREADS) keep_path_kernel(const KeepParams p) {
     __shared__ long long from[AHEAD], to[AHEAD];     // -1: nothing to move
+    __shared__ int kept;
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.y;
-    const int n = min(__ldcg(p.count + b), p.width);
-    if (n <= 1) return;
+    // The first warp alone asks for what all blocks of a request read, all at once.
+    int pos = 0, n = 0, next = 0;
+    if (threadIdx.x < 32) {
+        const int j = 1 + threadIdx.x % AHEAD;
+        n = min(__ldcg(p.count + b), p.width);
+        pos = __ldcg(p.pos_start + b);
+        next = j < p.width ? __ldcg(p.path + (size_t)b * p.width + j) : j;
+        if (threadIdx.x == 0) kept = n;
+    }
     const unsigned row = p.row_bytes / (unsigned)sizeof(V);
     const unsigned item = blockIdx.x * KEEP_THREADS + threadIdx.x;
     const unsigned r = item / row, plane = r / p.heads, layer = plane / p.planes;
-    char* base = p.cache + layer * p.layer_bytes + (plane - layer * p.planes) * p.plane_bytes + (r - plane * p.heads) * p.head_bytes +
-                 (item - r * row) * (unsigned)sizeof(V);
-    const int pos = __ldcg(p.pos_start + b);
-    for (int j0 = 1; j0 < n; j0 += AHEAD) {
-        if (j0 > 1) __syncthreads();                 // (the slots before have been read)
+    char* base = layer < p.layers ? p.cache + layer * p.layer_bytes + (plane - layer * p.planes) * p.plane_bytes + (r - plane * p.heads) * p.head_bytes +
+                 (item - r * row) * (unsigned)sizeof(V) : nullptr;
+    for (int j0 = 1;; j0 += AHEAD) {
         if (threadIdx.x < 2 * AHEAD) {
-            const int j = j0 + threadIdx.x % AHEAD, i = j < n ? __ldcg(p.path + (size_t)b * p.width + j) : j;
+            const int j = j0 + threadIdx.x % AHEAD;
+            if (j0 > 1 && j < n) next = __ldcg(p.path + (size_t)b * p.width + j);
+            const int i = j < n ? next : j;
             const long long at = (long long)pos + (threadIdx.x < AHEAD ? i : j);
             const unsigned entry = (unsigned)at / p.page_size;           // (at least 0, and below 2^32)
             long long place = -1;
@@ -97,14 +105,15 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_path_kernel(const KeepParam
             (threadIdx.x < AHEAD ? from : to)[threadIdx.x % AHEAD] = place;
         }
         __syncthreads();
-        if (layer >= p.layers) continue;
         V v[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
-            if (from[u] >= 0 && to[u] >= 0) v[u] = __ldcg((const V*)(base + from[u]));
+            if (from[u] >= 0 && to[u] >= 0 && base) v[u] = __ldcg((const V*)(base + from[u]));
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
-            if (from[u] >= 0 && to[u] >= 0) *(V*)(base + to[u]) = v[u];
+            if (from[u] >= 0 && to[u] >= 0 && base) *(V*)(base + to[u]) = v[u];
+        if (j0 + AHEAD >= kept) break;
+        __syncthreads();                             // (the slots have been read)
     }
 }
 
