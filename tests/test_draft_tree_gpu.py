@@ -396,6 +396,24 @@ def test_what_controls_leave_out(ops, kw):
     check_control(out, logits, given)
 
 
+@pytest.mark.parametrize("V", [601, 40961])
+def test_counts_of_long_histories(ops, V):
+    # more tokens than 15 bits count, one of them most of the time; a request of few beside it
+    rng = np.random.default_rng(V)
+    logits = torch.randn(5, V, generator=torch.Generator().manual_seed(V)) * 4
+    long = rng.permutation(np.concatenate([np.full(33000, V - 2), rng.integers(0, V, 7000)])).tolist()
+    settings = [(1.2, float(np.float32(2e-4)), 0.5), (1.1, 0.25, 0.0)]
+    trees, tokens = [[-1, 0, 0], [-1, 0]], np.array([V - 2, V - 2, 5, 3, 4])
+    requests = [(3, settings[0], long, 300, [(V - 2, 1.0)]), (2, settings[1], [3, 4, 3], 1, [])]
+    for tree in (False, True):
+        c = LogitControls(i32([0, 3, 5]), torch.tensor(settings, device=DEV), i32(long + [3, 4, 3]), i32([0, len(long)]), i32([len(long), 3]), i32([300, 1]),
+                          i32([0, 1, 1]), i32([V - 2]), torch.tensor([1.0], device=DEV), parents=i32(trees[0] + trees[1]) if tree else None,
+                          tokens=i32(tokens) if tree else None)
+        out = torch.empty_like(logits, device=DEV)
+        ops.control_logits(logits.to(DEV), out, c)
+        check_control(out, logits, (requests, trees if tree else None, tokens, None))
+
+
 def test_controls_of_the_largest_tree_and_of_rows_behind_the_last(ops):
     logits, c, given = controls_case(3, 700, [256, 0, 1], True)
     wide = torch.cat([logits, torch.full((2, 700), math.nan)]).to(DEV)
