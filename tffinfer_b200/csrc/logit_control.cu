@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
         __syncthreads();                             // (the part before is through with the counts)
         // The first history tokens, the masks of the first rows and the counts' zeros are on their way together.
         const int* at = p.history + first_token;
-        const int skew = (int)((uintptr_t)at >> 2 & 3), warp0 = tid & ~31;
+        const int skew = len > 0 ? (int)((uintptr_t)at >> 2 & 3) : 0, warp0 = tid & ~31;       // (without tokens nothing is loaded: the start may be any number)
         int4 t4[4];
         auto tokens_of = [&](int g0) {               // four tokens a load, from the 16 bytes on in which the history begins
 #pragma unroll
