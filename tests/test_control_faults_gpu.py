@@ -1,11 +1,13 @@
 """Controls of logits and draws at the edges of what they take."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
 import plain_tree as plain
 from tffinfer_b200.kernels.library import CudaKernels
-from tffinfer_b200.sampling import LogitControls
+from tffinfer_b200.sampling import LogitControls, Sampler, SamplingParams
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -41,3 +43,45 @@ def test_histories_that_are_none(ops):
             # two roundings, of values no larger than |x| * 1.5 + 0.5 * 3 + 0.25
             assert ((out.cpu().double() - want).abs() <= 2 * 2.0 ** -24 * (1.5 * logits.abs().double() + 1.75)).all()
             assert torch.equal(out.cpu()[:-1], logits[:-1])
+
+
+@pytest.mark.parametrize("penalty", [1.05, 1.2, 1.3, 0.7, 3.0, 1e-30])
+@pytest.mark.parametrize("V", [4001, 20000])
+def test_a_repetition_penalty_beside_other_controls(ops, penalty, V):
+    """A request's logits are the same, bit by bit, whether its neighbour has a bias or not."""
+    gen = torch.Generator().manual_seed(V)
+    rows = torch.randn(2, V, generator=gen) * 4
+    rows[0, ::7] *= 1e-38                           # some whose quotients or products are subnormal
+    seen = torch.randint(0, V, (1500,), generator=gen).tolist() + list(range(0, V, 49))
+    one = SamplingParams(repetition_penalty=penalty)
+    sampler = Sampler(ops, DEV)
+    got = []
+    for beside in (SamplingParams(), SamplingParams(logit_bias=((3, 1.5),)), SamplingParams(frequency_penalty=0.5)):
+        logits = rows.to(DEV)
+        drawn = sampler.sample(logits, [one, beside], [0, 1], [0, 0], [seen, [1, 2]], [0, 2])
+        got.append((logits[0].cpu(), int(drawn[0])))
+    want = rows[0].clone()
+    at = torch.tensor(sorted(set(seen)))
+    p = torch.tensor(penalty, dtype=torch.float32)
+    want[at] = torch.where(want[at] > 0, want[at] / p, want[at] * p)
+    for logits, drawn in got:
+        assert torch.equal(logits.view(torch.int32), want.view(torch.int32)) and drawn == got[0][1]
+
+
+@pytest.mark.parametrize("least,most", [(-126, 127), (-3, 3), (-40, -20), (20, 70)])
+def test_quotients_are_rounded_once(ops, least, most):
+    """Logits of every exponent and their special values, penalties of many: what a division in float32 gives, to the bit."""
+    rng = np.random.default_rng(abs(most))
+    R, V = 64, 4096
+    bits = rng.integers(0, 1 << 32, (R, V), dtype=np.uint32)
+    bits[R // 2:] = bits[R // 2:] & 0x7fffff | rng.integers(0x3a000000 >> 23, 0x44000000 >> 23, (R - R // 2, V), dtype=np.uint32) << 23    # 2^-11 to 2^9
+    x = torch.from_numpy(bits.view(np.float32).copy())
+    x[x.isnan()] = 1.5
+    x[:, 0], x[:, 1], x[:, 2], x[:, 3] = math.inf, -math.inf, 0.0, -0.0
+    penalties = torch.from_numpy((rng.uniform(1, 2, R) * 2.0 ** rng.integers(least, most + 1, R)).astype(np.float32))
+    settings = torch.stack([penalties, penalties * 0, penalties * 0], 1)
+    c = LogitControls(i32(range(R + 1)), settings.to(DEV), i32(range(V)), i32([0] * R), i32([V] * R), i32([0] * R))
+    out = torch.empty(R, V, device=DEV)
+    ops.control_logits(x.to(DEV), out, c)
+    want = torch.where(x > 0, x / penalties[:, None], x * penalties[:, None])
+    assert torch.equal(out.cpu().view(torch.int32), want.view(torch.int32))

@@ -17,9 +17,10 @@
 // What bounds it beside the traffic: instructions, and the warps that hide the way to memory.  A thread's addresses are a pointer and
 // an offset, and what a count does to a logit is worked out once for four rows, and not at all where none of a thread's four tokens was
 // seen (looked up and divided for every logit, 140 to 230 instructions for a warp's 128 of them, 256 rows of trees took 62 us and 64
-// rows 30).  Measured at a vocabulary of 151,936 with masks and 200 to 6,000 tokens of history: 64 rows 24.8 us (78 MB, 3.1
+// rows 30; as it was then).  Measured at a vocabulary of 151,936 with masks and 200 to 6,000 tokens of history: 64 rows 27.5 us (78 MB, 2.8
 // TB/s; a plain pass over as many bytes 13.4: the rest is what comes ahead of the first logits, 11,000 cycles of loads that wait for
-// one another), the 256 nodes of eight trees 56 (5.5 TB/s; 47), one row without a mask 5.2.
+// one another, and the quotients), the 256 nodes of eight trees 64.5 (4.8 TB/s; 47), one row without a mask 5.3.  The comparisons below are from before the
+// quotients were rounded once, with 24.9 and 56.
 //   Four CTAs an SM; with three, and larger slices, 29 and 62.  Tried without gain (64 rows, 256 nodes): the next loads ahead of a
 //   thread's work, 32 and 71 (registers for three CTAs an SM); a branch for each of a thread's tokens, 28 and 58; counted tokens put right behind a
 //   pass that only copies, 34 and 98; parts of rows by bulk copies through shared memory, 41 and 75 (half the instructions, too few warps).
@@ -67,17 +68,30 @@ struct Counts {
     }
 };
 
-// A request's penalties.  A positive logit of a token that was seen is multiplied by 1 / repetition, rounded once for the request: a second
-// rounding in float32 (2^-24) in place of a division an element.
+// Logits that are divided without the division's own instructions: from 2^-64 to 2^64, by penalties of 2^-32 to 2^32.
+constexpr unsigned LEAST_QUICK = 0x1f800000u, QUICK = 0x5f800000u - LEAST_QUICK;
+__device__ __noinline__ float divided(float x, float by) { return x / by; }
+
+// A request's penalties, with the operations of repetition_penalty_kernel (sampling.cu): a request's logits are the same, bit by bit,
+// whichever of the two kernels its step takes.  A quotient rounded once, at two products more than x * (1 / repetition) takes: with the
+// reciprocal y rounded to nearest, q = x y and the remainder r = x - q repetition (exact in an fma), q + r y is x / repetition
+// rounded to nearest where nothing over- or underflows (P. Markstein, Computation of elementary functions on the IBM RISC System/6000,
+// 1990).  64 rows 27.5 us, the nodes of eight trees 64.5; with a division for every such logit 28.1 and 72, with x y alone, a rounding more,
+// 24.9 and 56.
 struct Penalties {
     float rep, inverse, freq, pres;
+    unsigned quick;                                  // QUICK, or 0: this penalty is divided by
     // What is added to the logit of a token with this count (as Counts gives it): -0, which leaves all bits, where it was not generated.
     __device__ __forceinline__ float less(unsigned count) const {
         const unsigned n = count & 0x7fffffffu;
         return n ? -fmaf(freq, (float)n, pres) : -0.f;
     }
     __device__ __forceinline__ float apply(float x, bool seen, float less_) const {
-        return fmaf(x, seen ? x > 0.f ? inverse : rep : 1.f, less_);
+        const float q = x * inverse, quotient = fmaf(fmaf(-q, rep, x), inverse, q);
+        const bool in = __float_as_uint(x) - LEAST_QUICK < quick;
+        float y = in ? quotient : x * rep;
+        if (!in && x > 0.f) y = divided(x, rep);
+        return (seen ? y : x) + less_;
     }
     // ``more`` times on the row's path.
     __device__ __forceinline__ float operator()(float x, unsigned count, unsigned more = 0u) const {
@@ -114,6 +128,7 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
     const int prompt = own[7], e0 = max(0, own[8]), e1 = min(p.biases, own[9]);
     if (r0 >= r1) return;
     penalised.inverse = 1.f / penalised.rep;
+    penalised.quick = penalised.rep >= 0x1p-32f && penalised.rep <= 0x1p32f ? QUICK : 0u;
     const bool counted = penalised.rep != 1.f || penalised.freq != 0.f || penalised.pres != 0.f;
     const int len = !counted || first_token < 0 ? 0 : (int)max(0ll, min(held, p.history_size - first_token));
     Counts counts;
