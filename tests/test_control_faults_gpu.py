@@ -85,3 +85,25 @@ def test_quotients_are_rounded_once(ops, least, most):
     ops.control_logits(x.to(DEV), out, c)
     want = torch.where(x > 0, x / penalties[:, None], x * penalties[:, None])
     assert torch.equal(out.cpu().view(torch.int32), want.view(torch.int32))
+
+
+@pytest.mark.parametrize("nodes,kind", [([257], "random"), ([300, 2, 700], "random"), ([513], "chain"), ([1, 260], "star"), ([256, 257], "chain"), ([1100], "random")], ids=str)
+def test_trees_of_more_nodes_than_attention_takes(ops, nodes, kind):
+    """Every row of a tree gets its path's penalties, however many nodes the tree has."""
+    V, few, R = 333, 9, sum(nodes)
+    rng = np.random.default_rng(R)
+    logits = torch.randn(R, V, generator=torch.Generator().manual_seed(R)) * 4
+    trees = [list(range(-1, n - 1)) if kind == "chain" else [-1] + [0] * (n - 1) if kind == "star" else plain.random_tree(rng, n, spread=40, padding=n // 8) for n in nodes]
+    tokens = rng.integers(0, few, R)
+    settings = [(1.25, 0.0625, 0.5)] * len(nodes)
+    histories = [rng.integers(0, few, 20).tolist() for _ in nodes]
+    requests = [(n, s, h, 5, []) for n, s, h in zip(nodes, settings, histories)]
+    c = LogitControls(i32(np.concatenate([[0], np.cumsum(nodes)])), torch.tensor(settings, device=DEV), i32(np.concatenate(histories)),
+                      i32(np.arange(len(nodes)) * 20), i32([20] * len(nodes)), i32([5] * len(nodes)),
+                      parents=i32(np.concatenate(trees)), tokens=i32(tokens))
+    out = torch.empty(R, V, device=DEV)
+    ops.control_logits(logits.to(DEV), out, c)
+    want = plain.control(logits, requests, trees, tokens)
+    # three roundings, of values no larger than |x| * 1.25 + the penalties of all nodes and of the history
+    tol = 3 * 2.0 ** -24 * (1.25 * logits.abs().double() + 0.0625 * (max(nodes) + 20) + 0.5)
+    assert ((out.cpu().double() - want).abs() <= tol).all()

@@ -17,9 +17,9 @@
 // What bounds it beside the traffic: instructions, and the warps that hide the way to memory.  A thread's addresses are a pointer and
 // an offset, and what a count does to a logit is worked out once for four rows, and not at all where none of a thread's four tokens was
 // seen (looked up and divided for every logit, 140 to 230 instructions for a warp's 128 of them, 256 rows of trees took 62 us and 64
-// rows 30; as it was then).  Measured at a vocabulary of 151,936 with masks and 200 to 6,000 tokens of history: 64 rows 27.5 us (78 MB, 2.8
+// rows 30; as it was then).  Measured at a vocabulary of 151,936 with masks and 200 to 6,000 tokens of history: 64 rows 26.9 us (78 MB, 2.9
 // TB/s; a plain pass over as many bytes 13.4: the rest is what comes ahead of the first logits, 11,000 cycles of loads that wait for
-// one another, and the quotients), the 256 nodes of eight trees 64.5 (4.8 TB/s; 47), one row without a mask 5.3.  The comparisons below are from before the
+// one another, and the quotients), the 256 nodes of eight trees 62 (4.9 TB/s; 47), one row without a mask 5.3.  The comparisons below are from before the
 // quotients were rounded once, with 24.9 and 56.
 //   Four CTAs an SM; with three, and larger slices, 29 and 62.  Tried without gain (64 rows, 256 nodes): the next loads ahead of a
 //   thread's work, 32 and 71 (registers for three CTAs an SM); a branch for each of a thread's tokens, 28 and 58; counted tokens put right behind a
@@ -30,7 +30,7 @@
 namespace {
 
 constexpr int NT = 256, CTAS_AN_SM = 4;
-constexpr int MAX_NODES = 256;                       // of a request's tree
+constexpr int NODES = 256;                           // of a request's tree in shared memory: a larger one's others are read where they lie
 constexpr int ROWS_AT_ONCE = 256;
 constexpr int MOST_TOKENS = 17408, LEAST_TOKENS = 1024;        // of a slice: 34 KB of counts beside the rest's 20 leave room for four CTAs an SM
 constexpr int MASK_WORDS = 2304;                     // of masks in shared memory: a part of the rows' at a time
@@ -105,10 +105,10 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
     extern __shared__ unsigned count_words[];        // [slice / 2]
     __shared__ int mask_at[ROWS_AT_ONCE];
     __shared__ unsigned masks[MASK_WORDS];           // of a part of the rows: [row][words of the slice]
-    __shared__ short parent[MAX_NODES];
-    __shared__ int token[MAX_NODES];
+    __shared__ short parent[NODES];
+    __shared__ int token[NODES];
     __shared__ unsigned short lists[NT / 32][512];   // a warp's tokens of the slice: their places, and a bit for the prompt's
-    __shared__ short hits[MAX_NODES];                // nodes whose tokens lie in the slice
+    __shared__ short hits[NODES];                    // nodes whose tokens lie in the slice, of NODES at a time
     __shared__ int hit_count, bias_range[2];
     __shared__ int own[10];                          // the request's: rows, penalties, history, biases
     pdl_launch_dependents();
@@ -134,12 +134,17 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
     Counts counts;
     counts.words = count_words;
     counts.wide = len > 32767;
-    const int nodes = p.parents && counted ? min(r1 - r0, MAX_NODES) : 0;
-    for (int i = tid; i < nodes; i += NT) {
+    const int nodes = p.parents && counted ? r1 - r0 : 0;
+    auto parent_at = [&](int i) -> int {
         const int up = __ldcg(p.parents + r0 + i);
-        parent[i] = (short)(up < -1 || up >= i ? -2 : up);
+        return up < -1 || up >= i ? -2 : up;
+    };
+    for (int i = tid; i < min(nodes, NODES); i += NT) {
+        parent[i] = (short)parent_at(i);
         token[i] = __ldcg(p.tokens + r0 + i);
     }
+    auto parent_of = [&](int i) -> int { return i < NODES ? parent[i] : parent_at(i); };
+    auto token_of = [&](int i) { return i < NODES ? token[i] : __ldcg(p.tokens + r0 + i); };
     auto mask_of = [&](int r) {
         const int m = p.mask ? (p.mask_row ? __ldcg(p.mask_row + r) : r) : -1;
         return m < p.mask_rows ? m : -1;
@@ -199,8 +204,11 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
             if (biased >= lo && biased < hi) { atomicMin(&bias_range[0], e); atomicMax(&bias_range[1], e + 1); }
             biased = e + NT < e1 ? __ldcg(p.bias_tokens + e + NT) : -1;
         }
-        for (int i = tid; i < nodes; i += NT)
-            if (token[i] >= lo && token[i] < hi) hits[atomicAdd(&hit_count, 1)] = (short)i;
+        auto hits_of = [&](int u0) {                 // which of nodes u0 .. have a token of the slice
+            for (int i = u0 + tid; i < min(nodes, u0 + NODES); i += NT)
+                if (token_of(i) >= lo && token_of(i) < hi) hits[atomicAdd(&hit_count, 1)] = (short)(i - u0);
+        };
+        hits_of(0);
         if (masked) mask_words_of(min(at_once, r1 - r0));
         // Few tokens are the slice's: a warp lists those of its 512 and then counts them a lane each.  (With a branch for every token
         // nearly every one was taken by some lane.)
@@ -367,24 +375,36 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
         }
 
         // ------------------------------------------------ what paths and biases change
-        if (nodes > 0) {
-            __syncthreads();
-            // a thread a node of the slice's and a node that may have it on its path; a token that is there more than once is done where
-            // the path has it first, for all of them
+        // a thread a node of the slice's and a node that may have it on its path; a token that is there more than once is done where
+        // the path has it first, for all of them
+        auto paths_of = [&](int u0, auto parent_of, auto token_of) {
             for (int i = tid; i < hit_count * nodes; i += NT) {
-                const int up = hits[i / nodes], node = i % nodes, t = token[up];
+                const int up = u0 + hits[i / nodes], node = i % nodes, t = token_of(up);
                 int o = node;
                 bool first = true;
-                while (o > up) { first = first && token[o] != t; o = parent[o]; }
+                while (o > up) { first = first && token_of(o) != t; o = parent_of(o); }
                 if (o != up || !first) continue;
                 unsigned more = 1;
-                for (o = parent[up]; o >= 0; o = parent[o]) more += token[o] == t;
+                for (o = parent_of(up); o >= 0; o = parent_of(o)) more += token_of(o) == t;
                 if (o != -1) continue;               // padding, or a node behind it: no path
                 const size_t k = (size_t)(r0 + node) * p.vocab + t;
                 const float x = __ldcg(p.logits + k);
                 if (allowed(r0 + node, t)) p.out[k] = penalised(x, len > 0 ? counts.at(t - lo) : 0u, more);
             }
-        }
+        };
+        if (nodes > 0) __syncthreads();
+        if (nodes <= NODES) paths_of(0, [&](int i) -> int { return parent[i]; }, [&](int i) { return token[i]; });
+        else
+            for (int u0 = 0; u0 < nodes; u0 += NODES) {
+                if (u0 > 0) {
+                    __syncthreads();
+                    if (tid == 0) hit_count = 0;
+                    __syncthreads();
+                    hits_of(u0);
+                    __syncthreads();
+                }
+                paths_of(u0, parent_of, token_of);
+            }
         const int f0 = bias_range[0], f1 = bias_range[1], n_rows = r1 - r0;
         if (f0 < f1) {
             __syncthreads();

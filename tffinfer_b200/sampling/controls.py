@@ -35,8 +35,9 @@ class LogitControls:
     mask [M, words], mask_row [R]
                                 bit t % 32 of word t // 32: token t is allowed.  Row r has mask mask_row[r], none if that is
                                 not in [0, M); without mask_row it has mask r
-    parents [R], tokens [R]     the rows of a request are the nodes of a tree of drafted tokens (at most 256): parents as in
-                                ``CudaKernels.attention_tree``.  A row's path is its node and that node's ancestors
+    parents [R], tokens [R]     the rows of a request are the nodes of a tree of drafted tokens: parents as in
+                                ``CudaKernels.attention_tree``, and as many as there are (a tree of more than 256 takes longer a
+                                node).  A row's path is its node and that node's ancestors
     """
     row_start: torch.Tensor
     settings: torch.Tensor
