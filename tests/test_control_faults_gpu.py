@@ -107,3 +107,18 @@ def test_trees_of_more_nodes_than_attention_takes(ops, nodes, kind):
     # three roundings, of values no larger than |x| * 1.25 + the penalties of all nodes and of the history
     tol = 3 * 2.0 ** -24 * (1.25 * logits.abs().double() + 0.0625 * (max(nodes) + 20) + 0.5)
     assert ((out.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("biases,masked,want", [
+    ([(5, 3e38), (5, 3e38), (5, -math.inf)], False, -math.inf), ([(5, -math.inf), (5, 3e38), (5, 3e38)], False, -math.inf),
+    ([(5, 3e38), (5, 3e38)], True, -math.inf), ([(5, 2.0), (5, -math.inf)], True, -math.inf), ([(5, 3e38), (5, -3e38)], False, 1.0),
+    ([(5, 3e38), (5, 3e38)], False, math.inf)], ids=str)
+def test_biases_of_one_token_that_add_up_beyond_float32(ops, biases, masked, want):
+    logits = torch.ones(1, 64, device=DEV)
+    mask = np.full((1, 2), -1, dtype=np.int32)
+    mask[0, 0] = ~np.int32(1 << 5)
+    c = LogitControls(i32([0, 1]), torch.tensor([[1.0, 0.0, 0.0]], device=DEV), i32([]), i32([0]), i32([0]), i32([0]), i32([0, len(biases)]),
+                      i32([t for t, _ in biases]), torch.tensor([v for _, v in biases], device=DEV), i32(mask) if masked else None)
+    out = torch.empty_like(logits)
+    ops.control_logits(logits, out, c)
+    assert float(out[0, 5]) == want and (out[0, :5] == 1).all() and (out[0, 6:] == 1).all()
