@@ -413,16 +413,16 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
                 const int e = f0 + (int)(i / n_rows), r = r0 + (int)(i % n_rows);
                 const int t = __ldcg(p.bias_tokens + e);
                 if (t < lo || t >= hi || (e > e0 && __ldcg(p.bias_tokens + e - 1) == t)) continue;
-                float bias = 0.f;
-                bool banned = false;
-                for (int o = e; o < e1 && __ldcg(p.bias_tokens + o) == t; ++o) {
+                float* to = p.out + (size_t)r * p.vocab + t;
+                const float x = *to;
+                float bias = __ldcg(p.bias_values + e);
+                bool banned = bias == -INFINITY;
+                for (int o = e + 1; o < e1 && __ldcg(p.bias_tokens + o) == t; ++o) {
                     const float v = __ldcg(p.bias_values + o);
                     banned = banned || v == -INFINITY;
                     bias += v;
                 }
                 // (finite ones may add up to infinity, which frees no token that a mask or a bias bans)
-                float* to = p.out + (size_t)r * p.vocab + t;
-                const float x = *to;
                 *to = banned || x == -INFINITY ? -INFINITY : x + bias;
             }
         }
