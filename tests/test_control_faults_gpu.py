@@ -122,3 +122,96 @@ def test_biases_of_one_token_that_add_up_beyond_float32(ops, biases, masked, wan
     out = torch.empty_like(logits)
     ops.control_logits(logits, out, c)
     assert float(out[0, 5]) == want and (out[0, :5] == 1).all() and (out[0, 6:] == 1).all()
+
+
+def draws_in_the_middle(row, T=1.0):
+    """(tokens, numbers): numbers that lie in the middle of the kept tokens' stretches, by sums in 64 bits."""
+    e = torch.exp((row.double() - row.max()) / T)
+    ends = torch.cumsum(e, 0) / e.sum()
+    kept = torch.nonzero(e > 0.0)[:, 0]
+    u = (ends - e / e.sum() / 2)[kept].float()
+    wide = (e / e.sum())[kept] > 1e-5             # (narrower ones lie within the rounding of the sums)
+    return kept[wide], u[wide]
+
+
+@pytest.mark.parametrize("V", [500, 32768, 151936])
+@pytest.mark.parametrize("allowed,k", [(1, 50), (3, 50), (49, 50), (50, 50), (51, 50), (200, 50)])
+def test_top_k_of_rows_with_few_allowed_tokens(ops, V, allowed, k):
+    gen = torch.Generator().manual_seed(V + allowed)
+    row = torch.randn(V, generator=gen)
+    keep = torch.randperm(V, generator=gen)[:allowed]
+    banned = torch.full((V,), -math.inf)
+    banned[keep] = row[keep]
+    top = torch.full((V,), -math.inf)
+    best = torch.topk(banned, min(k, allowed)).indices
+    top[best] = banned[best]
+    tokens, u = draws_in_the_middle(top)
+    R = tokens.numel()
+    out = torch.empty(R, dtype=torch.int32, device=DEV)
+    one = torch.ones(R, device=DEV)
+    ops.sample(banned.repeat(R, 1).to(DEV), one, u.to(DEV), out, top_k=i32([k] * R), top_p=one, min_p=one * 0)
+    assert out.tolist() == tokens.tolist()
+
+
+def test_top_k_where_most_allowed_tokens_lie_far_below(ops):
+    """Fewer than k tokens above e^-32 of the largest; with the largest taken away, the cut is what it would be without it."""
+    V, k = 4096, 4
+    row = torch.full((V,), -math.inf)
+    row[7], row[100], row[200], row[300], row[400], row[500] = 0.0, -40.0, -41.0, -42.0, -43.0, -44.0
+    for T, cut in ((1.0, None), (20.0, 4)):         # at T = 20 all lie within e^-3: the cut is seen
+        top = row.clone()
+        if cut:
+            top[400] = top[500] = -math.inf
+        tokens, u = draws_in_the_middle(top, T)
+        R = tokens.numel()
+        out = torch.empty(R, dtype=torch.int32, device=DEV)
+        one = torch.ones(R, device=DEV)
+        ops.sample(row.repeat(R, 1).to(DEV), one * T, u.to(DEV), out, top_k=i32([k] * R), top_p=one, min_p=one * 0)
+        assert out.tolist() == tokens.tolist()
+
+
+def test_rows_that_allow_nothing_give_the_first_token(ops):
+    logits = torch.full((3, 40000), -math.inf, device=DEV)
+    out = torch.full((3,), 9, dtype=torch.int32, device=DEV)
+    one = torch.ones(3, device=DEV)
+    for filters in ({}, dict(top_k=i32([50] * 3), top_p=one, min_p=one * 0), dict(top_k=i32([0] * 3), top_p=one * 0.9, min_p=one * 0.1)):
+        ops.sample(logits, one, one * 0.5, out, **filters)
+        assert out.tolist() == [0, 0, 0]
+
+
+def test_a_grammar_does_not_make_top_k_slow(ops):
+    """A row with fewer allowed tokens than k takes no longer than one whose tokens are all allowed (twice as long, for the clock's noise)."""
+    V, R = 151936, 8
+    gen = torch.Generator().manual_seed(1)
+    open_ = (torch.randn(R, V, generator=gen) * 4).to(DEV)
+    held = torch.full((R, V), -math.inf, device=DEV)
+    held[:, :20] = open_[:, :20]
+    out = torch.empty(R, dtype=torch.int32, device=DEV)
+    one = torch.ones(R, device=DEV)
+    def best(logits):
+        times = []
+        for _ in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            ops.sample(logits, one, one * 0.5, out, top_k=i32([50] * R), top_p=one, min_p=one * 0)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+    for logits in (held, torch.full_like(held, -math.inf)):
+        t, limit = best(logits), 2 * best(open_)
+        assert t <= limit, (t, limit)
+
+
+def test_masks_that_leave_many(ops):
+    """More allowed tokens than the list of candidates takes, most of them far below the largest; either filter, and both."""
+    V = 40000
+    row = torch.full((V,), -math.inf)
+    row[1000:13000] = -40.0
+    row[500] = 0.0
+    logits = row.repeat(3, 1).to(DEV)
+    one = torch.ones(3, device=DEV)
+    out = torch.empty(3, dtype=torch.int32, device=DEV)
+    for top_p in (1.0, 0.9):
+        ops.sample(logits, one, one * 0.5, out, top_k=i32([50, 20000, 0]), top_p=one * top_p, min_p=one * 0)
+        assert out.tolist() == [500, 500, 500]
