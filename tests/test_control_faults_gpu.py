@@ -215,3 +215,18 @@ def test_masks_that_leave_many(ops):
     for top_p in (1.0, 0.9):
         ops.sample(logits, one, one * 0.5, out, top_k=i32([50, 20000, 0]), top_p=one * top_p, min_p=one * 0)
         assert out.tolist() == [500, 500, 500]
+
+
+def test_an_infinite_logit_is_drawn(ops):
+    V = 40000
+    for rest in (-math.inf, 1.0):
+        row = torch.full((V,), rest)
+        row[123] = math.inf
+        logits = row.repeat(2, 1).to(DEV)
+        one = torch.ones(2, device=DEV)
+        out = torch.empty(2, dtype=torch.int32, device=DEV)
+        ops.sample(logits, one, one * 0.5, out)
+        assert out.tolist() == [123, 123]
+        for k, p in ((50, 1.0), (0, 0.9), (50, 0.9), (20000, 0.99)):
+            ops.sample(logits, one, one * 0.5, out, top_k=i32([k] * 2), top_p=one * p, min_p=one * 0)
+            assert out.tolist() == [123, 123]

@@ -266,7 +266,13 @@ sample_kernel(const float* __restrict__ logits, const float* __restrict__ temper
                     if (round == 0) total_mass = running;
                 }
                 if (pick < 0) pick = last_kept;                        // rounding left the target at the very end
-                if (tid == 0) out[r] = pick >= 0 ? pick : 0;
+                if (tid == 0) {
+                    if (pick < 0) {                                    // nothing is kept beside an infinite maximum: take it
+                        pick = 0;
+                        for (int i = 0; i < vocab; ++i) if (row[i] == mx) { pick = i; break; }
+                    }
+                    out[r] = pick;
+                }
             }
             return;
         }
