@@ -63,10 +63,14 @@ class SamplingParams:
                 or self.token_mask is not None)
 
     @property
+    def needs_generated_tokens(self) -> bool:
+        """Whether a draw depends on which tokens the request has generated (rather than had)."""
+        return self.frequency_penalty != 0.0 or self.presence_penalty != 0.0 or self.token_mask is not None
+
+    @property
     def needs_token_values(self) -> bool:
         """Whether a draw depends on which tokens the request has had."""
-        return (self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0 or self.presence_penalty != 0.0
-                or self.token_mask is not None)
+        return self.repetition_penalty != 1.0 or self.needs_generated_tokens
 
     @property
     def is_greedy(self) -> bool:

@@ -51,10 +51,10 @@ class Sampler:
         if R == 0:
             return out
         if any(p.controls_logits for p in params):
-            if (seen_tokens is None or prompt_lens is None) and any(p.needs_token_values for p in params):
+            if (seen_tokens is None or prompt_lens is None) and any(p.needs_generated_tokens for p in params):
                 raise ValueError("a penalty or a grammar needs the requests' tokens and how many of them are the prompt")
             seen = [list(t) if p.needs_token_values else [] for p, t in zip(params, seen_tokens or [[]] * R)]
-            lens = [n if p.needs_token_values else 0 for p, n in zip(params, prompt_lens or [0] * R)]
+            lens = [n if p.needs_generated_tokens else 0 for p, n in zip(params, prompt_lens or [0] * R)]
             self.ops.control_logits(logits, logits, LogitControls.of(params, lens, seen, logits.shape[1], logits.device))
         elif any(p.repetition_penalty != 1.0 for p in params):
             self._penalize(logits, params, seen_tokens)
