@@ -31,3 +31,15 @@ def test_a_repetition_penalty_beside_a_bias_needs_no_prompt_length():
     for p in (SamplingParams(repetition_penalty=1.5, presence_penalty=0.1), SamplingParams(token_mask=lambda made: None)):
         with pytest.raises(ValueError, match="needs the requests' tokens"):
             Sampler(ops, "cpu").sample(torch.zeros(2, 4), [p, params[1]], [0, 1], [0, 0], [[2, 3], []])
+
+
+@pytest.mark.parametrize("penalty", [1e39, float("inf"), float("nan"), 1e-46, 0.0, -1.0])
+def test_repetition_penalties_that_float32_does_not_hold(penalty):
+    """An infinite one makes a logit of 0 NaN, one that rounds to 0 every positive logit infinite."""
+    with pytest.raises(ValueError, match="repetition_penalty"):
+        SamplingParams(repetition_penalty=penalty)
+
+
+@pytest.mark.parametrize("penalty", [1.0, 3e38, 2e-45, 0.5])
+def test_repetition_penalties_that_float32_holds(penalty):
+    assert SamplingParams(repetition_penalty=penalty).repetition_penalty == penalty

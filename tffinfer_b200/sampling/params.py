@@ -47,8 +47,8 @@ class SamplingParams:
             raise ValueError("temperature must be >= 0")
         if self.top_k < 0 or not (0 < self.top_p <= 1.0) or not (0 <= self.min_p < 1.0):
             raise ValueError("top_k >= 0, 0 < top_p <= 1 and 0 <= min_p < 1 are required")
-        if self.repetition_penalty <= 0:
-            raise ValueError("repetition_penalty must be > 0")
+        if not 0 < self.repetition_penalty <= _FLOAT32_MAX or np.float32(self.repetition_penalty) == 0:
+            raise ValueError("repetition_penalty must be > 0 and finite in float32")
         if not (abs(self.frequency_penalty) <= _FLOAT32_MAX and abs(self.presence_penalty) <= _FLOAT32_MAX):
             raise ValueError("frequency_penalty and presence_penalty must be finite in float32")
         if any(not 0 <= t < 2**31 or not v <= _FLOAT32_MAX for t, v in self.logit_bias):
