@@ -16,7 +16,7 @@ import torch
 
 from .. import log
 from ..config import EngineConfig
-from ..sampling import Sampler, SamplingParams
+from ..sampling import Sampler, SamplingParams, mask_of
 from .batch import StepEntry
 from .runner import ModelRunner
 from .scheduler import Scheduler, Request, StepOutput, PENDING
@@ -105,7 +105,7 @@ class Engine:
                 logits, [r.params for r in samplers], [r.key for r in samplers],
                 [len(r.generated) for r in samplers],
                 [r.tokens for r in samplers] if need_seen else None,
-                [len(r.prompt) for r in samplers])
+                [len(r.prompt) for r in samplers], self._masks(plan))
             record["tokens"] = toks
             if toks.is_cuda:
                 i = self._host_flip                    # two pinned buffers in turn: the one of the step
@@ -133,6 +133,24 @@ class Engine:
         if not self.ecfg.async_steps:
             outs += self._resolve_inflight()
         return outs
+
+    def _masks(self, plan):
+        """What the grammars of the step's sampling requests allow, or None where none has one.  A request whose grammar fails draws
+        nothing and ends with this step; the others know nothing of it."""
+        entries = [e for e in plan.entries if e.samples]
+        if all(e.request.params.token_mask is None for e in entries):
+            return None
+        masks = []
+        for e in entries:
+            r, mask = e.request, None
+            if r.params.token_mask is not None and len(r.generated) < r.params.max_new_tokens:
+                try:
+                    mask = mask_of(r.params, r.generated, self.runner.desc.vocab_size)
+                except Exception as err:
+                    log.error("request %r ends behind its %d tokens, its grammar failed: %s: %s", r.id, len(r), type(err).__name__, err)
+                    e.reason = "bad_mask"
+            masks.append(mask)
+        return masks
 
     def _needs_token_values(self) -> bool:
         return any(r.params.needs_token_values for r in self.scheduler.running) or \

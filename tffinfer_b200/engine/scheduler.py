@@ -18,6 +18,7 @@ Policy
     its pages and slot go back, it keeps its tokens (prompt + generated) and moves to
     the FRONT of the waiting queue, to be recomputed from the start; the draw for a
     token depends on (seed, request, index) only, so its output does not change;
+  * a request whose grammar fails finishes with reason "bad_mask";
   * a request that cannot fit even alone finishes with reason "out_of_memory";
     a prompt longer than the model allows is refused with reason "too_long"
     (the reference truncates with a warning, InferRuntime.cu:399-403).
@@ -181,7 +182,9 @@ class Scheduler:
                 self.counters["prefill_tokens"] += len(e.tokens)
             if not e.samples:
                 continue
-            if len(r.generated) >= r.params.max_new_tokens:
+            if e.reason is not None:
+                pass                                   # its grammar failed: nothing is drawn
+            elif len(r.generated) >= r.params.max_new_tokens:
                 e.reason = "length"                    # nothing is drawn
             else:
                 r.generated.append(PENDING)

@@ -14,6 +14,18 @@ import torch
 from .params import SamplingParams
 
 
+def mask_of(params: SamplingParams, made: Sequence[int], vocab: int) -> Optional[np.ndarray]:
+    """What the grammar of ``params`` allows behind the generated tokens ``made``: 32-bit words, or None for no limit.  Raises what the
+    grammar raises, and ValueError for anything else that it gives."""
+    mask = params.token_mask(list(made)) if params.token_mask is not None else None
+    if mask is None:
+        return None
+    mask, words = np.ascontiguousarray(mask), -(-vocab // 32)
+    if mask.dtype.itemsize != 4 or mask.dtype.kind not in "iu" or mask.shape != (words,):
+        raise ValueError(f"a token mask is {words} 32-bit words for {vocab} tokens, got {mask.dtype} {mask.shape}")
+    return mask
+
+
 @dataclass
 class LogitControls:
     """The controls of a step's logit rows, tensors on the device (int32 unless said otherwise).  B requests, R rows.
@@ -81,18 +93,17 @@ class LogitControls:
 
     @classmethod
     def of(cls, params: Sequence[SamplingParams], prompts: Sequence[int], histories: Sequence[Sequence[int]], vocab: int,
-           device) -> "LogitControls":
-        """The controls of one row a request: its settings, the length of its prompt and its tokens so far."""
+           device, masks: Optional[Sequence[Optional[np.ndarray]]] = None) -> "LogitControls":
+        """The controls of one row a request: its settings, the length of its prompt and its tokens so far.  ``masks``: what the
+        requests' grammars have given already (``mask_of``); None: they are asked here."""
         B = len(params)
         lens = np.fromiter((len(h) for h in histories), dtype=np.int64, count=B)
         start = np.concatenate([[0], np.cumsum(lens)])
         biases = [sorted(p.logit_bias) for p in params]
         count = np.concatenate([[0], np.cumsum([len(x) for x in biases])])
-        masks = [p.token_mask(list(h[n:])) if p.token_mask is not None else None for p, n, h in zip(params, prompts, histories)]
-        words, held = -(-vocab // 32), [np.ascontiguousarray(m) for m in masks if m is not None]
-        for m in held:
-            if m.dtype.itemsize != 4 or m.dtype.kind not in "iu" or m.shape != (words,):
-                raise ValueError(f"a token mask is {words} 32-bit words for {vocab} tokens, got {m.dtype} {m.shape}")
+        if masks is None:
+            masks = [mask_of(p, h[n:], vocab) for p, n, h in zip(params, prompts, histories)]
+        words, held = -(-vocab // 32), [m for m in masks if m is not None]
         row = np.cumsum([m is not None for m in masks]) - 1
         row[[m is None for m in masks]] = -1
         # one buffer of 32-bit words, one copy

@@ -41,11 +41,13 @@ class Sampler:
 
     def sample(self, logits: torch.Tensor, params: Sequence[SamplingParams], request_keys: Sequence[int],
                indices: Sequence[int], seen_tokens: Optional[Sequence[Sequence[int]]] = None,
-               prompt_lens: Optional[Sequence[int]] = None) -> torch.Tensor:
+               prompt_lens: Optional[Sequence[int]] = None,
+               masks: Optional[Sequence[Optional[np.ndarray]]] = None) -> torch.Tensor:
         """logits float32 [R, V]; row r belongs to a request with params[r], key request_keys[r],
         generating its token number indices[r]; seen_tokens[r] (prompt + generated) is needed only
         when a penalty or a grammar is set (params[r].needs_token_values), prompt_lens[r] (how many of
-        them are the prompt) only for another one than the repetition penalty.  Returns int32 [R] on the device."""
+        them are the prompt) only for another one than the repetition penalty.  ``masks``: what the rows' grammars allow, where
+        they have been asked already (controls.mask_of).  Returns int32 [R] on the device."""
         R = logits.shape[0]
         out = torch.empty(R, dtype=torch.int32, device=logits.device)
         if R == 0:
@@ -55,7 +57,7 @@ class Sampler:
                 raise ValueError("a penalty or a grammar needs the requests' tokens and how many of them are the prompt")
             seen = [list(t) if p.needs_token_values else [] for p, t in zip(params, seen_tokens or [[]] * R)]
             lens = [n if p.needs_generated_tokens else 0 for p, n in zip(params, prompt_lens or [0] * R)]
-            self.ops.control_logits(logits, logits, LogitControls.of(params, lens, seen, logits.shape[1], logits.device))
+            self.ops.control_logits(logits, logits, LogitControls.of(params, lens, seen, logits.shape[1], logits.device, masks))
         elif any(p.repetition_penalty != 1.0 for p in params):
             self._penalize(logits, params, seen_tokens)
         if all(p.is_greedy for p in params):
