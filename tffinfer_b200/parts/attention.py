@@ -21,6 +21,8 @@ import torch
 from ..registry import register_part
 from .base import Mixer, SplitMixer, WeightSpec, MATRIX, VECTOR, KVNeed, StateNeed, LayerContext
 
+TREE_FILES = ("attention_tree", "attention_tree_tc")     # a step over trees of drafted tokens (CudaKernels.attention_tree)
+
 
 @register_part("mixer", "gqa_attention")
 class GQAttention(Mixer):
@@ -45,7 +47,7 @@ class GQAttention(Mixer):
         self.w_qkv = self.w_o = self.q_norm_w = self.k_norm_w = None
 
     def kernel_files(self):
-        return ("attention_bf16", "attention_decode", "attention_prefill", "attention_generic")
+        return ("attention_bf16", "attention_decode", "attention_prefill", "attention_generic") + TREE_FILES
 
     def cache_need(self):
         return KVNeed(self.num_kv_heads, self.head_dim, self.window)
@@ -171,7 +173,7 @@ class GatedSinkAttention(Mixer):
         self.conv_w = self.conv_wt = self.norm_w = self.bias = None
 
     def kernel_files(self):
-        files = ("attention_bf16", "attention_decode", "attention_prefill", "attention_generic", "qkv_finish", "streams")
+        files = ("attention_bf16", "attention_decode", "attention_prefill", "attention_generic", "qkv_finish", "streams") + TREE_FILES
         return files if getattr(self, "head_finish", False) else files + ("short_conv",)
 
     def cache_need(self):
