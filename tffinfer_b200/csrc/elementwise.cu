@@ -303,12 +303,14 @@ TFF_API int tff_rope_table(float* table, const float* inv_freq, int max_pos, int
 // Per-head norm before RoPE: src/core/model/qwen3/QWen3Creator.cpp:93-101; rotate-half
 // pairing (i, i + rot/2): src/kernel/cuda/paged_flash_attention.cu:300-384; cache write:
 // src/kernel/cuda/set_row.cu:72-123.  Unlike the reference, keys are stored rotated.
+// ``slots``: the cache slot of every token, where it is another one than its position's (nodes of a tree, whose siblings have one
+// position); null: the position's.
 template <typename TIN, typename T>
 __global__ void qk_norm_rope_kv_write_kernel(
     TIN* __restrict__ qkv, int clear_input, T* __restrict__ q_out,
     const float* __restrict__ q_w, const float* __restrict__ k_w, float eps,
     const float2* __restrict__ table, int rot_dim,
-    const int* __restrict__ positions, const int* __restrict__ tok_req,
+    const int* __restrict__ positions, const int* __restrict__ slots, const int* __restrict__ tok_req,
     const int* __restrict__ block_table, int table_width,
     T* __restrict__ cache, KvLayout L, int layer, int write_cache,
     int nq, int nkv, int d, int max_pos) {
@@ -333,13 +335,14 @@ __global__ void qk_norm_rope_kv_write_kernel(
     } else {
         const int kvh = is_k ? head - nq : head - nq - nkv;
         const int b = tok_req[t];
-        const int page = block_table[(size_t)b * table_width + pos / L.page_size];
+        const int at = slots ? slots[t] : pos;
+        const int page = block_table[(size_t)b * table_width + at / L.page_size];
         if (page < 0) {                       // no page: the host never schedules this; write nothing
             if (clear_input) for (int i = lane; i < d; i += 32) src[i] = from_f32<TIN>(0.f);
             return;
         }
         dst = cache + (size_t)page * L.page_stride + (size_t)layer * L.layer_stride +
-              (is_k ? 0 : L.kv_stride) + (size_t)kvh * L.head_stride + (size_t)(pos % L.page_size) * d;
+              (is_k ? 0 : L.kv_stride) + (size_t)kvh * L.head_stride + (size_t)(at % L.page_size) * d;
     }
     if (!is_q && !is_k) {                     // V: plain copy
         for (int i = lane; i < d; i += 32) {
@@ -394,7 +397,7 @@ qk_norm_rope_kv_write_d128_kernel(
     float* __restrict__ qkv, int clear_input, T* __restrict__ q_out,
     const float* __restrict__ q_w, const float* __restrict__ k_w, float eps,
     const float2* __restrict__ table,
-    const int* __restrict__ positions, const int* __restrict__ tok_req,
+    const int* __restrict__ positions, const int* __restrict__ slots, const int* __restrict__ tok_req,
     const int* __restrict__ block_table, int table_width,
     T* __restrict__ cache, KvLayout L, int layer, int write_cache, int nq, int nkv, int max_pos) {
     pdl_launch_dependents();
@@ -415,10 +418,11 @@ qk_norm_rope_kv_write_d128_kernel(
         dst = q_out + (size_t)t * nq * d + (size_t)head * d + lane * 4;
     } else if (wanted) {
         const int kvh = is_k ? head - nq : head - nq - nkv;
-        const int page = block_table[(size_t)tok_req[t] * table_width + pos / L.page_size];
+        const int at = slots ? slots[t] : pos;
+        const int page = block_table[(size_t)tok_req[t] * table_width + at / L.page_size];
         if (page >= 0)
             dst = cache + (size_t)page * L.page_stride + (size_t)layer * L.layer_stride +
-                  (is_k ? 0 : L.kv_stride) + (size_t)kvh * L.head_stride + (size_t)(pos % L.page_size) * d + lane * 4;
+                  (is_k ? 0 : L.kv_stride) + (size_t)kvh * L.head_stride + (size_t)(at % L.page_size) * d + lane * 4;
     }
     const float* w = is_q ? q_w : (is_k ? k_w : nullptr);
     float4 wv = make_float4(1.f, 1.f, 1.f, 1.f);
@@ -459,7 +463,7 @@ qk_norm_rope_kv_write_d128_kernel(
 TFF_API int tff_qk_norm_rope_kv_write(
     void* qkv, int in_is_f32, int clear_input, void* q_out, int is_bf16, const float* q_w, const float* k_w, float eps,
     const float* table, int rot_dim, int max_pos,
-    const int* positions, const int* tok_req, const int* block_table, int table_width,
+    const int* positions, const int* slots, const int* tok_req, const int* block_table, int table_width,
     void* cache, int cache_layers, int layer, int page_size, int write_cache,
     int num_tokens, int nq, int nkv, int d, cudaStream_t stream) {
     if (num_tokens <= 0) return TFF_OK;
@@ -472,17 +476,17 @@ TFF_API int tff_qk_norm_rope_kv_write(
         dim3 grid8((heads + 7) / 8, num_tokens);
         if (is_bf16)
             return tff_launch_pdl(qk_norm_rope_kv_write_d128_kernel<bf16>, grid8, dim3(256), 0, stream, (float*)qkv,
-                                  clear_input, (bf16*)q_out, q_w, k_w, eps, (const float2*)table, positions, tok_req,
+                                  clear_input, (bf16*)q_out, q_w, k_w, eps, (const float2*)table, positions, slots, tok_req,
                                   block_table, table_width, (bf16*)cache, L, layer, write_cache, nq, nkv, max_pos);
         return tff_launch_pdl(qk_norm_rope_kv_write_d128_kernel<float>, grid8, dim3(256), 0, stream, (float*)qkv,
-                              clear_input, (float*)q_out, q_w, k_w, eps, (const float2*)table, positions, tok_req,
+                              clear_input, (float*)q_out, q_w, k_w, eps, (const float2*)table, positions, slots, tok_req,
                               block_table, table_width, (float*)cache, L, layer, write_cache, nq, nkv, max_pos);
     }
     const int warps = 4;
     dim3 grid((heads + warps - 1) / warps, num_tokens);
 #define TFF_QK_LAUNCH(TIN, T)                                                                                  \
     tff_launch_pdl(qk_norm_rope_kv_write_kernel<TIN, T>, grid, warps * 32, 0, stream,                          \
-        (TIN*)qkv, clear_input, (T*)q_out, q_w, k_w, eps, (const float2*)table, rot_dim, positions, tok_req,          \
+        (TIN*)qkv, clear_input, (T*)q_out, q_w, k_w, eps, (const float2*)table, rot_dim, positions, slots, tok_req,          \
         block_table, table_width, (T*)cache, L, layer, write_cache, nq, nkv, d, max_pos)
     if (is_bf16) {
         if (in_is_f32) return TFF_QK_LAUNCH(float, bf16);

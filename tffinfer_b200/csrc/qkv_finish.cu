@@ -17,7 +17,8 @@
 // the gates, and v where there is a cache to take it): the row is then an accumulator buffer that the next split
 // product adds into.
 // The cache is [pages, layers, 2, kv heads, page, dc] with dc >= max(d, dv): keys use the first d elements of a
-// slot, values the first dv.
+// slot, values the first dv.  ``slots_of``: the slot of every token, where it is another one than its position's (nodes of a tree,
+// whose siblings have one position); null: the position's.
 // Everything is computed in float32; only the stores round.
 #include "common.cuh"
 
@@ -27,7 +28,7 @@ template <typename TIN, typename TQ, typename TC>
 __global__ void __launch_bounds__(128)
 qkv_finish_kernel(TIN* __restrict__ proj, int clear_input, int ld, TQ* __restrict__ q_out, float* __restrict__ k_out,
                   const float* __restrict__ freq, int rot_dims, float magnitude, int interleaved, float k_scale,
-                  const int* __restrict__ positions, const int* __restrict__ tok_req,
+                  const int* __restrict__ positions, const int* __restrict__ slots_of, const int* __restrict__ tok_req,
                   const int* __restrict__ block_table, int table_width,
                   TC* __restrict__ cache, KvLayout L, int layer, int dc,
                   int v_mode, float* __restrict__ v_share, const float* __restrict__ lambda,
@@ -55,10 +56,11 @@ qkv_finish_kernel(TIN* __restrict__ proj, int clear_input, int ld, TQ* __restric
     TC* slot = nullptr;
     if (!is_q && cache != nullptr) {
         const int kvh = is_k ? head - nq : head - nq - nkv;
-        const int page = block_table[(size_t)tok_req[t] * table_width + pos / L.page_size];
+        const int at = slots_of ? slots_of[t] : pos;
+        const int page = block_table[(size_t)tok_req[t] * table_width + at / L.page_size];
         if (page < 0) return;                                     // no page: the host never schedules this
         slot = cache + (size_t)page * L.page_stride + (size_t)layer * L.layer_stride + (is_k ? 0 : L.kv_stride) +
-               (size_t)kvh * L.head_stride + (size_t)(pos % L.page_size) * dc;
+               (size_t)kvh * L.head_stride + (size_t)(at % L.page_size) * dc;
     }
     if (!is_q && !is_k) {                                         // a value head
         const int kvh = head - nq - nkv;
@@ -139,7 +141,7 @@ __global__ void __launch_bounds__(QF_WARPS * 32)
 qk_finish4_kernel(float* __restrict__ proj, int clear_input, int ld, TQ* __restrict__ q_out, const float* __restrict__ qw,
                   const float* __restrict__ kw, float eps, const float* __restrict__ bias, int v_is_k,
                   const float* __restrict__ freq, int rot_dims, float magnitude,
-                  const int* __restrict__ positions, const int* __restrict__ tok_req, const int* __restrict__ block_table,
+                  const int* __restrict__ positions, const int* __restrict__ slots_of, const int* __restrict__ tok_req, const int* __restrict__ block_table,
                   int table_width, TQ* __restrict__ cache, KvLayout L, int layer, int dc, int nq, int nkv, int d) {
     __shared__ float4 cs[16], sn[16];
     pdl_launch_dependents();
@@ -150,8 +152,9 @@ qk_finish4_kernel(float* __restrict__ proj, int clear_input, int ld, TQ* __restr
         sincosf((float)pos * freq[threadIdx.x], &s, &c);
         reinterpret_cast<float*>(sn)[threadIdx.x] = s * magnitude; reinterpret_cast<float*>(cs)[threadIdx.x] = c * magnitude;
     }
-    const int page = block_table[(size_t)tok_req[t] * table_width + pos / L.page_size];
-    TQ* slots = cache + (size_t)page * L.page_stride + (size_t)layer * L.layer_stride + (size_t)(pos % L.page_size) * dc;
+    const int at = slots_of ? slots_of[t] : pos;
+    const int page = block_table[(size_t)tok_req[t] * table_width + at / L.page_size];
+    TQ* slots = cache + (size_t)page * L.page_stride + (size_t)layer * L.layer_stride + (size_t)(at % L.page_size) * dc;
     const bool on = lane < d4;
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), one = make_float4(1.f, 1.f, 1.f, 1.f);
     const float4 wq = on && qw ? reinterpret_cast<const float4*>(qw)[lane] : one;
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(QF_WARPS * 32)
 qk_finish_kernel(float* __restrict__ proj, int clear_input, int ld, TQ* __restrict__ q_out, const float* __restrict__ qw,
                  const float* __restrict__ kw, float eps, const float* __restrict__ bias, int v_is_k,
                  const float* __restrict__ freq, int rot_dims, float magnitude, int interleaved,
-                 const int* __restrict__ positions, const int* __restrict__ tok_req, const int* __restrict__ block_table,
+                 const int* __restrict__ positions, const int* __restrict__ slots_of, const int* __restrict__ tok_req, const int* __restrict__ block_table,
                  int table_width, TQ* __restrict__ cache, KvLayout L, int layer, int dc, int nq, int nkv, int d, int dv) {
     __shared__ float cs[QF_MOST_D / 2], sn[QF_MOST_D / 2];
     constexpr int PJ = (RJ + 1) / 2;
@@ -249,10 +252,11 @@ qk_finish_kernel(float* __restrict__ proj, int clear_input, int ld, TQ* __restri
     const bool is_q = head < nq, is_k = !is_q && head < nq + nkv;
     TQ* slot = nullptr;                                           // the head's key slot (a value lies kv_stride further)
     if (!is_q && head < nq + (v_is_k ? nkv : 2 * nkv)) {
-        const int page = block_table[(size_t)tok_req[t] * table_width + pos / L.page_size];
+        const int at = slots_of ? slots_of[t] : pos;
+        const int page = block_table[(size_t)tok_req[t] * table_width + at / L.page_size];
         if (page >= 0)                                            // no page: the host never schedules this
             slot = cache + (size_t)page * L.page_stride + (size_t)layer * L.layer_stride +
-                   (size_t)(is_k ? head - nq : head - nq - nkv) * L.head_stride + (size_t)(pos % L.page_size) * dc;
+                   (size_t)(is_k ? head - nq : head - nq - nkv) * L.head_stride + (size_t)(at % L.page_size) * dc;
     }
     pdl_wait();
     if (!is_q && !slot) return;
@@ -316,7 +320,7 @@ qk_finish_kernel(float* __restrict__ proj, int clear_input, int ld, TQ* __restri
 // bias float32 over the row's columns or null; v_is_k: the row has no value columns, dv = d.
 TFF_API int tff_qk_finish(
     float* proj, int clear_input, int ld, void* q_out, int q_dt, const float* qw, const float* kw, float eps, const float* bias,
-    int v_is_k, const float* freq, int rot_dims, float magnitude, int interleaved, const int* positions, const int* tok_req,
+    int v_is_k, const float* freq, int rot_dims, float magnitude, int interleaved, const int* positions, const int* slots_of, const int* tok_req,
     const int* block_table, int table_width, void* cache, int cache_layers, int layer, int page_size, int dc,
     int num_tokens, int nq, int nkv, int d, int dv, cudaStream_t stream) {
     if (num_tokens <= 0) return TFF_OK;
@@ -335,7 +339,7 @@ TFF_API int tff_qk_finish(
         const dim3 grid4(num_tokens > 256 ? 1 : (nq + nkv + QF_WARPS - 1) / QF_WARPS, num_tokens);
 #define TFF_QF4(TQ)                                                                                                   \
         return tff_launch_pdl(qk_finish4_kernel<TQ>, grid4, dim3(QF_WARPS * 32), 0, stream, proj, clear_input, ld, (TQ*)q_out, \
-                              qw, kw, eps, bias, v_is_k, freq, rot_dims, magnitude, positions, tok_req, block_table,  \
+                              qw, kw, eps, bias, v_is_k, freq, rot_dims, magnitude, positions, slots_of, tok_req, block_table,  \
                               table_width, (TQ*)cache, L, layer, dc, nq, nkv, d)
         if (q_dt == 1) TFF_QF4(bf16);
         TFF_QF4(float);
@@ -343,7 +347,7 @@ TFF_API int tff_qk_finish(
     }
 #define TFF_QF(TQ, RJ)                                                                                                \
     return tff_launch_pdl(qk_finish_kernel<TQ, RJ>, grid, dim3(QF_WARPS * 32), 0, stream, proj, clear_input, ld, (TQ*)q_out, \
-                          qw, kw, eps, bias, v_is_k, freq, rot_dims, magnitude, interleaved, positions, tok_req,      \
+                          qw, kw, eps, bias, v_is_k, freq, rot_dims, magnitude, interleaved, positions, slots_of, tok_req,      \
                           block_table, table_width, (TQ*)cache, L, layer, dc, nq, nkv, d, dv)
     if (q_dt == 1) { if (d <= 128) TFF_QF(bf16, 4); TFF_QF(bf16, 16); }
     if (d <= 128) TFF_QF(float, 4);
@@ -355,7 +359,7 @@ TFF_API int tff_qk_finish(
 TFF_API int tff_qkv_finish(
     void* proj, int in_dt, int clear_input, int ld, void* q_out, int q_dt, float* k_out,
     const float* freq, int rot_dims, float magnitude, int interleaved, float k_scale,
-    const int* positions, const int* tok_req, const int* block_table, int table_width,
+    const int* positions, const int* slots_of, const int* tok_req, const int* block_table, int table_width,
     void* cache, int cache_dt, int cache_layers, int layer, int page_size, int dc,
     int v_mode, float* v_share, const float* lambda, int gate_off, float* gate_out,
     int num_tokens, int nq, int nkv, int d, int dv, const float* bias, float unit_eps, cudaStream_t stream) {
@@ -374,7 +378,7 @@ TFF_API int tff_qkv_finish(
     dim3 grid((heads + 3) / 4, num_tokens);
 #define TFF_FIN(TIN, TQ, TC)                                                                                       \
     return tff_launch_pdl(qkv_finish_kernel<TIN, TQ, TC>, grid, dim3(128), 0, stream, (TIN*)proj, clear_input, ld, (TQ*)q_out, \
-                          k_out, freq, rot_dims, magnitude, interleaved, k_scale, positions, tok_req, block_table,   \
+                          k_out, freq, rot_dims, magnitude, interleaved, k_scale, positions, slots_of, tok_req, block_table,   \
                           table_width, (TC*)cache, L, layer, dc, v_mode, v_share, lambda, gate_off, gate_out, nq,     \
                           nkv, d, dv, bias, unit_eps)
     if (in_dt == 0 && q_dt == 0 && cache_dt == 0) TFF_FIN(float, float, float);

@@ -14,6 +14,7 @@ requests bring one token at position 0 whose keys go to a page nobody reads.
 """
 from __future__ import annotations
 
+import dataclasses
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple
 
@@ -33,6 +34,7 @@ class StepEntry:
                                                  # id from on the device, or -1 for the id given in ``tokens``
 
 
+MAX_TREE_NODES = 256     # of a request's tree of drafted tokens
 NUM_FLAT = 10     # flat integer arrays ahead of the block tables in the packed buffer
 
 
@@ -92,6 +94,36 @@ class StepBatch:
     real_requests: int = 0        # requests that are not padding
     real_logit_rows: int = 0
     graph_bucket: Optional[int] = None   # set when the arrays are the fixed ones of a CUDA-graph bucket
+    # A step over trees of drafted tokens (``with_parents``): every token's parent among its request's tokens of this step, and the cache
+    # slot that its keys and values are written to (None: positions).  Siblings have one position and a slot each.
+    parents: Optional[torch.Tensor] = None       # int32 [T]
+    cache_slots: Optional[torch.Tensor] = None   # int32 [T]
+
+    def with_parents(self, parents: Sequence[Sequence[int]]) -> "StepBatch":
+        """This step with each request's tokens as the nodes of a tree: ``parents[b][i]`` is an earlier node of request b, -1 for a node
+        that follows the request's cached tokens, anything else (-2) for padding, which sees nothing and is seen by none.  Node i
+        keeps the cache slot that token i has; its position is the cached tokens plus its ancestors."""
+        if self.graph_bucket is not None:
+            raise ValueError("a step over trees has arrays of its own, not those of a captured step")
+        counts = np.asarray(self.h_q_lens, dtype=np.int64)
+        if [len(p) for p in parents] != counts.tolist():
+            raise ValueError(f"a request's parents are a number for each of its tokens: {[len(p) for p in parents]} for {counts.tolist()}")
+        if counts.size and counts.max() > MAX_TREE_NODES:
+            raise ValueError(f"a request brings at most {MAX_TREE_NODES} nodes, got {int(counts.max())}")
+        first = np.repeat(np.cumsum(counts) - counts, counts)
+        up = np.fromiter((int(x) for p in parents for x in p), dtype=np.int64, count=int(counts.sum()))
+        node = np.arange(up.size) - first
+        up = np.where((up < -1) | (up >= node), -2, up)
+        depth, at = np.zeros(up.size, dtype=np.int64), up.copy()
+        while (at >= 0).any():                       # an ancestor further for every node
+            depth += at >= 0
+            at = np.where(at >= 0, up[np.where(at >= 0, first + at, 0)], at)
+        depth[at != -1] = 0                          # (a chain that ends in padding: the node is not there)
+        arrays = np.concatenate([up, np.repeat(np.asarray(self.h_pos_start, dtype=np.int64), counts) + depth]).astype(np.int32)
+        host = torch.from_numpy(arrays)
+        device = self.positions.device
+        dev = host.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else host
+        return dataclasses.replace(self, parents=dev[:up.size], positions=dev[up.size:], cache_slots=self.positions)
 
 
 def batch_views(dev: torch.Tensor, layout: BatchLayout):

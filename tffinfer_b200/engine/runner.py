@@ -21,7 +21,7 @@ from ..config import EngineConfig, read_config_json
 from ..parts import Model, CacheBinding, KVNeed, StateNeed
 from ..registry import get_architecture
 from ..weights import load_model_weights
-from .batch import StepEntry, StepBatch, packed_to_device, batch_from_device, BatchLayout
+from .batch import StepEntry, StepBatch, packed_to_device, batch_from_device, BatchLayout, MAX_TREE_NODES
 
 _TORCH_DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 _STATE_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": torch.int32}
@@ -183,12 +183,25 @@ class ModelRunner:
         return self.cache.num_tokens(req)
 
     # ------------------------------------------------------------------- step
-    def make_batch(self, entries: Sequence[StepEntry], prev_tokens: Optional[torch.Tensor] = None) -> StepBatch:
+    def make_batch(self, entries: Sequence[StepEntry], prev_tokens: Optional[torch.Tensor] = None,
+                   parents: Optional[Sequence[Sequence[int]]] = None) -> StepBatch:
         """Checks the entries, takes the pages they need (all or nothing) and builds
         the device-side batch.  Raises OutOfPages without side effects.  Entries with
-        ``token_src`` take token ids from ``prev_tokens`` (int32, on the device)."""
+        ``token_src`` take token ids from ``prev_tokens`` (int32, on the device).
+
+        ``parents``: the entries' tokens are the nodes of trees (``StepBatch.with_parents``), node 0 the token drawn last.  Behind
+        ``run_batch`` the draws say which are kept (``accept_tree``); their slots are moved in every cache group (``keep_path``) and
+        ``cache.commit(request, kept)`` counts them."""
+        if parents is not None:
+            problem = self.model.trees_problem()
+            if problem is not None:
+                raise RequestError(f"this model takes no trees of drafted tokens: {problem}")
+            if len(parents) != len(entries) or any(len(p) != len(e.tokens) for p, e in zip(parents, entries)):
+                raise RequestError("parents are a list an entry, with a number a token")
+            if any(len(p) > MAX_TREE_NODES for p in parents):
+                raise RequestError(f"a request brings at most {MAX_TREE_NODES} nodes")
         arrays = self._check_and_reserve(entries, prev_tokens)
-        if self._graph_eligible(entries):
+        if parents is None and self._graph_eligible(entries):
             batch = self._make_static_batch(entries, arrays)
             if batch.tok_src is not None:
                 self.ops.gather_tokens(batch.token_ids, prev_tokens, batch.tok_src)
@@ -199,6 +212,9 @@ class ModelRunner:
         self.last_h2d_bytes = batch.token_ids.numel() * 0 + 4 * (
             3 * batch.num_tokens + 4 * batch.num_requests + 1 + batch.num_logit_rows
             + sum(t.numel() for t in batch.block_tables))
+        if parents is not None:
+            batch = batch.with_parents(parents)
+            self.last_h2d_bytes += 8 * batch.num_tokens
         return batch
 
     def _check_and_reserve(self, entries, prev_tokens):

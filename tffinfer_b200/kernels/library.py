@@ -197,6 +197,21 @@ class CudaKernels:
             raise KernelError(f"a tensor of {t.dtype} where the kernel takes {dtype}")
 
     @staticmethod
+    def _slots_of(batch, T: int):
+        """Where the keys and values of a step's tokens are written, if that is not where their positions say (StepBatch.cache_slots)."""
+        slots = getattr(batch, "cache_slots", None)
+        if slots is not None:
+            CudaKernels._need_here(_I32, (slots,))
+            if slots.numel() != T:
+                raise KernelError(f"cache slots are {T} numbers, one a token")
+        return slots
+
+    @staticmethod
+    def _need_chains(batch) -> None:
+        if getattr(batch, "parents", None) is not None:
+            raise KernelError("the tokens of this step are nodes of trees: attention_tree takes them, this kernel does not")
+
+    @staticmethod
     def _cache_args(kv_cache, kv_layer: int):
         """(pointer, pages, layers, layer) of a paged cache [pages, layers, 2, kv heads, page, head] as the
         launchers take them.  The tensor is either contiguous as it reads (pages outermost), or that shape
@@ -707,7 +722,7 @@ class CudaKernels:
             _vp(proj.data_ptr() + proj_off * proj.element_size()), _c_int(_dt(proj)), _c_int(clear), _c_int(ld), _ptr(q_out),
             _c_int(_dt(q_out)), _ptr(k_out),
             _ptr(f), _c_int(rot), _c_float(mag), _c_int(1 if inter else 0), _c_float(k_scale),
-            _ptr(batch.positions), _ptr(batch.tok_req), _ptr(block_table),
+            _ptr(batch.positions), _ptr(self._slots_of(batch, T)), _ptr(batch.tok_req), _ptr(block_table),
             _c_int(block_table.shape[1] if block_table is not None else 0),
             c_ptr, _c_int(_dt(kv_cache)) if kv_cache is not None else _c_int(0), _c_int(c_layers), _c_int(c_layer),
             _c_int(page_size), _c_int(dc), _c_int(v_mode), _ptr(v_share), _ptr(lam), _c_int(gate_off), _ptr(gate_out),
@@ -739,7 +754,7 @@ class CudaKernels:
         self._check(self.lib.tff_qk_finish(
             _ptr(proj), _c_int(clear), _c_int(ld), _ptr(q_out), _c_int(_dt(q_out)), _ptr(qw), _ptr(kw), _c_float(eps),
             _ptr(bias), _c_int(1 if values_are_keys else 0), _ptr(f), _c_int(rot), _c_float(mag), _c_int(1 if inter else 0),
-            _ptr(batch.positions), _ptr(batch.tok_req), _ptr(block_table), _c_int(block_table.shape[1]), c_ptr,
+            _ptr(batch.positions), _ptr(self._slots_of(batch, T)), _ptr(batch.tok_req), _ptr(block_table), _c_int(block_table.shape[1]), c_ptr,
             _c_int(c_layers), _c_int(c_layer), _c_int(page_size), _c_int(kv_cache.shape[-1]), _c_int(T), _c_int(nq),
             _c_int(nkv), _c_int(d), _c_int(dv), self._stream()), "qk_finish")
         if clear and last_reader:
@@ -760,6 +775,11 @@ class CudaKernels:
         (with ``heads``): rows whose first columns hold the product already; somebody else reads the others behind this."""
         if not write_cache:
             raise KernelError("attend_gated writes the keys and values it attends to; a borrowed cache is not supported")
+        parents = getattr(batch, "parents", None)
+        if pre is not None and parents is not None:
+            raise KernelError("a convolution over time or a norm of the whole projection is not built for steps over trees")
+        # (a step over trees: the same arguments, and the nodes' parents)
+        attention = self.attention_ext if parents is None else functools.partial(self._attention_nodes, parents)
         T = h.shape[0]
         if isinstance(h, DeferredNorm):
             h = h.materialize()
@@ -773,8 +793,7 @@ class CudaKernels:
             self.qk_finish(proj, q, heads.get("norm"), float(heads.get("eps", 0.0)), heads.get("bias"),
                            bool(heads.get("values_are_keys")), freq, batch, block_table, kv_cache, kv_layer, page_size, nq,
                            nkv, d, dv, last_reader)
-            self.attention_ext(q, batch, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window,
-                               softcap, sink, gates, keep)
+            attention(q, batch, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window, softcap, sink, gates, keep)
             return
         if pre is not None:
             taps = int(pre.get("taps") or 1)
@@ -798,8 +817,10 @@ class CudaKernels:
             proj = mixed
         self.qkv_finish(proj, q, None, freq, batch, block_table, kv_cache, kv_layer, page_size, nq, nkv, d, dv,
                         1.0, v_mode, v_share, lam, gate_off, gates)
-        self.attention_ext(q, batch, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window,
-                           softcap, sink, gates)
+        attention(q, batch, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, dv, scale, window, softcap, sink, gates)
+
+    def _attention_nodes(self, parents, q, batch, *args) -> None:
+        self.attention_tree(q, batch, parents, *args)
 
     @staticmethod
     def _sink_args(sink, nq: int):
@@ -816,6 +837,7 @@ class CudaKernels:
         with a cap on the scores, a sink in the softmax (True: of score 0; a float32 tensor [nq]: of that score per head)
         and a multiplier per (token, head).  ``keep``: beside a window, the first so many positions stay visible."""
         self._need_cuda(q, block_table, out, gates)
+        self._need_chains(batch)
         T = q.shape[0]
         dc = kv_cache.shape[-1]
         assert kv_cache.dtype == q.dtype == out.dtype
@@ -855,7 +877,8 @@ class CudaKernels:
         pos_start[b], its ancestors' and its own.  ``parents`` int32 [T]: an earlier node of the request, or -1 for a node that
         follows the cached tokens.  A node whose chain of parents does not end at -1 (padding: -2) sees nothing, is seen by
         none, and gives zeros.  A node's position, which counts for ``window`` and ``keep``, is pos_start[b] + its
-        ancestors (the queries and keys are rotated by it: ``batch.positions`` of such a step).  At most 256 nodes a request.
+        ancestors (the queries and keys are rotated by it: ``batch.positions`` of such a step, made by ``StepBatch.with_parents``,
+        whose ``cache_slots`` say where the kernels that write keys and values put them).  At most 256 nodes a request.
         The keys and values of cached tokens and of nodes that are there are finite; padding's may be anything."""
         T, B, dtype = q.shape[0], batch.num_requests, q.dtype
         dc = kv_cache.shape[-1]
@@ -2064,7 +2087,7 @@ class CudaKernels:
             _ptr(qkv), _c_int(1 if qkv.dtype == torch.float32 else 0), _c_int(clear), _ptr(q_out), _c_int(_dt(q_out)),
             _ptr(q_w), _ptr(k_w), _c_float(eps),
             _ptr(table), _c_int(rot_dim), _c_int(table.shape[0] if table is not None else 0),
-            _ptr(batch.positions), _ptr(batch.tok_req), _ptr(block_table),
+            _ptr(batch.positions), _ptr(self._slots_of(batch, T)), _ptr(batch.tok_req), _ptr(block_table),
             _c_int(block_table.shape[1] if block_table is not None else 0),
             c_ptr, _c_int(c_layers), _c_int(c_layer), _c_int(page_size), _c_int(1 if write_cache else 0),
             _c_int(T), _c_int(nq), _c_int(nkv), _c_int(d), self._stream()), "qk_norm_rope_kv_write")
@@ -2082,9 +2105,9 @@ class CudaKernels:
         T, K = h.shape
         if isinstance(h, DeferredNorm):
             h = h.materialize()
-        # The fused form runs on pairs of SMs only.  Where another configuration saves more waves than the separate
+        # The fused form runs on pairs of SMs only, and writes keys and values where the positions say.  Where another configuration saves more waves than the separate
         # kernel costs (a pass over the float32 projection at about 5 TB/s and a launch), the projection is not fused.
-        if self.USE_SM_PAIRS and T > self.SWAP_MAX_M:
+        if self.USE_SM_PAIRS and T > self.SWAP_MAX_M and getattr(batch, "cache_slots", None) is None:
             costs = self.prompt_costs(T, (nq + 2 * nkv) * d, K, False)
             apart = min(v[0] for v in costs.values()) + T * (nq + 2 * nkv) * d * 6 / 5e6 + 3.0
             pairs_pay = 512 in costs and costs[512][0] <= apart
@@ -2125,17 +2148,23 @@ class CudaKernels:
         attention (with the merge of its key shares).  A decode attention that took the projection's float32
         accumulators and finished queries, new keys and new values itself was built and measured: one launch
         fewer and 0.05 ms a step slower at the Qwen3-8B shape (under programmatic dependent launch the small
-        kernel's time already hid behind the attention's first loads of old keys), so it was not kept."""
+        kernel's time already hid behind the attention's first loads of old keys), so it was not kept.
+        The attention of a step over trees (batch.parents) is attention_tree."""
         T = h.shape[0]
         q = torch.empty((T, nq * d), dtype=out.dtype, device=out.device)
         self.qkv_project(h, w_qkv, q, q_w, k_w, eps, table, rot_dim, batch, block_table, kv_cache, kv_layer, page_size,
                          nq, nkv, d, write_cache)
+        parents = getattr(batch, "parents", None)
+        if parents is not None:
+            self.attention_tree(q, batch, parents, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, d, scale, window)
+            return
         self.attention(q, batch, block_table, kv_cache, kv_layer, page_size, out, nq, nkv, d, scale, window)
 
     def attention(self, q, batch, block_table, kv_cache, kv_layer, page_size, out,
                   nq, nkv, d, scale, window) -> None:
         """q [T, nq*d] (normed, rotated) against the paged cache -> out [T, nq*d]."""
         self._need_cuda(q, block_table, out)
+        self._need_chains(batch)
         T = q.shape[0]
         assert kv_cache.dtype == q.dtype == out.dtype
         assert tuple(q.shape) == (T, nq * d) and tuple(out.shape) == (T, nq * d)

@@ -46,6 +46,8 @@ class GQAttention(Mixer):
         self.kv_width = self.num_kv_heads * self.head_dim
         self.w_qkv = self.w_o = self.q_norm_w = self.k_norm_w = None
 
+    takes_trees = True
+
     def kernel_files(self):
         return ("attention_bf16", "attention_decode", "attention_prefill", "attention_generic") + TREE_FILES
 
@@ -243,6 +245,10 @@ class GatedSinkAttention(Mixer):
     @property
     def takes_projection(self) -> bool:
         return self.head_finish
+
+    @property
+    def takes_trees(self) -> bool:
+        return self.conv_taps == 0 and self.qk_norm != "whole"
 
     def forward(self, h, ctx: LayerContext, residual, proj=None):
         ops, batch = ctx.ops, ctx.batch

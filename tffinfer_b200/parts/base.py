@@ -147,6 +147,7 @@ class Mixer(Part):
     output_bias = None    # float32 [hidden] of the output projection, or None.  With ``residual`` None the output comes
                           # WITHOUT it: the arrangement adds it where it joins the output to the residual
 
+    takes_trees = False   # whether a step's tokens may be nodes of trees (StepBatch.parents): each sees its ancestors and the cached tokens
     w_in = None           # the rows of the mixer's input product, where it ...
     takes_projection = False     # ... says that forward(h, ctx, None, proj=rows) takes that product from the first columns of
                                  # ``rows`` (an arrangement that runs it together with products of its own; the other columns

@@ -86,6 +86,16 @@ class Model:
             files.add("streams")
         return sorted(files)
 
+    def trees_problem(self) -> Optional[str]:
+        """Why a step of this model cannot run over trees of drafted tokens, or None: every mixer has to see a token's ancestors in
+        place of the tokens ahead of it, and so has what reads the tokens before at the embedding."""
+        for b in self.blocks:
+            if not b.mixer.takes_trees:
+                return f"its mixer '{b.mixer.kind}' reads the tokens ahead of a token in their order"
+        if self.embed_extras:
+            return f"its embedding '{self.embed_extras[0].kind}' reads the tokens ahead of a token in their order"
+        return None
+
     def load(self, tensors: Dict[str, torch.Tensor], ops, act_dtype: torch.dtype, device) -> None:
         d = self.desc
         self.embed = tensors[d.embed_name]
