@@ -19,6 +19,14 @@ import sys
 import time
 
 
+def _parse_bias(text: str):
+    token, colon, value = text.partition(":")
+    try:
+        return int(token), float(value)
+    except ValueError:
+        raise argparse.ArgumentTypeError(f"a bias is TOKEN:VALUE, got '{text}'") from None
+
+
 def build_parser() -> argparse.ArgumentParser:
     ap = argparse.ArgumentParser(prog="tffinfer_b200", description=__doc__,
                                  formatter_class=argparse.RawDescriptionHelpFormatter)
@@ -39,6 +47,10 @@ def build_parser() -> argparse.ArgumentParser:
     s.add_argument("--top-p", type=float, default=1.0, help="_top_p (1 = off)")
     s.add_argument("--min-p", type=float, default=0.0, help="_min_p (0 = off)")
     s.add_argument("--repetition-penalty", type=float, default=1.0, help="_repetition_penalty (1 = off)")
+    s.add_argument("--frequency-penalty", type=float, default=0.0, help="taken off a token's logit for every time it was generated")
+    s.add_argument("--presence-penalty", type=float, default=0.0, help="taken off a token's logit once it was generated")
+    s.add_argument("--logit-bias", type=_parse_bias, action="append", default=[], metavar="TOKEN:VALUE",
+                   help="added to a token's logit; -inf bans it (repeatable)")
     s.add_argument("--seed", type=int, default=0, help="_seed")
     s.add_argument("--eos", type=int, action="append", default=[], help="token id that ends a request (repeatable)")
     p = ap.add_argument_group("prompts (token ids; the engine has no tokenizer)")
@@ -70,11 +82,22 @@ def _parse_ids(text: str):
     return [int(t) for t in text.replace(",", " ").split()]
 
 
+def sampling_params(args):
+    """The sampling options of a parsed command line."""
+    from tffinfer_b200.sampling import SamplingParams
+    temperature = args.temperature if args.temperature is not None else (0.0 if args.sample_type in (None, "greedy") else 1.0)
+    if args.sample_type == "greedy":
+        temperature = 0.0
+    return SamplingParams.make(temperature=temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p,
+                               repetition_penalty=args.repetition_penalty, frequency_penalty=args.frequency_penalty,
+                               presence_penalty=args.presence_penalty, logit_bias=tuple(args.logit_bias), seed=args.seed,
+                               max_new_tokens=args.n_predict, eos_token_ids=tuple(args.eos))
+
+
 def main(argv=None) -> int:
     args = build_parser().parse_args(argv)
     import tffinfer_b200 as tff
     from tffinfer_b200.config import EngineConfig
-    from tffinfer_b200.sampling import SamplingParams
 
     if args.random_config:
         if not args.save_model:
@@ -119,12 +142,7 @@ def main(argv=None) -> int:
         print("no prompt given (--prompt-ids, --prompt-file or --prompt-len)", file=sys.stderr)
         return 2
 
-    temperature = args.temperature if args.temperature is not None else (0.0 if args.sample_type in (None, "greedy") else 1.0)
-    if args.sample_type == "greedy":
-        temperature = 0.0
-    sp = SamplingParams.make(temperature=temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p,
-                             repetition_penalty=args.repetition_penalty, seed=args.seed,
-                             max_new_tokens=args.n_predict, eos_token_ids=tuple(args.eos))
+    sp = sampling_params(args)
     t0 = time.time()
     if args.kernel_trace:
         from tffinfer_b200.kernels.trace import KernelTrace
