@@ -25,7 +25,8 @@
 // cycles, about what the memory gives an SM: 64 trees of 8 nodes behind 200 to 6,000 tokens (32/8 heads) 148 us, 5.4 TB/s.  With two tiles it takes
 // 1,590, the products' and exponentials' time: a tree of 64 nodes behind 32,000 tokens (64/8 heads) 83 to 95 us by the clock
 // that the power cap leaves.  Around that, a CTA's first scores come 7,500 to 10,000 cycles after its start (2,900 for its place in the line, 3,500 for the
-// first keys), and a second piece costs about six blocks: 8 trees of 32 nodes behind 2,048 tokens 26.5 us, 71 MB.
+// first keys), and a second piece costs about six blocks: 8 trees of 32 nodes behind 2,048 tokens 25.4 us, 71 MB.  Two tiles leave a thread 96
+// registers, and 92 bytes are spilled (heads of 128; 80 with heads of 64, none with one tile).
 //   - The queries go ahead of all but two blocks of keys: behind a full ring of every CTA's they came 7,000 cycles later.
 //   - A walk counts ``extra`` = 6 units more than its blocks: 3 gives 94.4 / 27.8 us (the long tree / the 8 trees), 5 and 7 92.3, 91.2 / 27.2, 27.3, and
 //     12 91.2 / 28.7.
