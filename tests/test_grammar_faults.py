@@ -85,3 +85,18 @@ def test_a_grammar_is_not_asked_for_a_token_that_is_not_drawn(tmp_path):
         return None
     assert eng.generate([[1, 2, 3]], SamplingParams(max_new_tokens=0, token_mask=mask)) == [[]] and asked == []
     assert len(eng.generate([[1, 2, 3]], SamplingParams(max_new_tokens=4, token_mask=mask))[0]) == 4 and asked == [0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+def test_a_grammar_that_reuses_its_array(tmp_path, backend):
+    """One grammar serves two requests from one array, which it fills anew at each call: each request has its own mask."""
+    eng, shared = _engine(tmp_path, backend), np.zeros(WORDS, np.int32)
+    def parity(odd):
+        def mask(made):
+            bits = np.zeros(WORDS * 32, dtype=bool)
+            bits[odd::2] = True
+            shared[:] = np.packbits(bits, bitorder="little").view(np.int32)
+            return shared
+        return mask
+    got = eng.generate([[1, 2, 3], [4, 5]], [SamplingParams(max_new_tokens=5, token_mask=parity(0)), SamplingParams(max_new_tokens=5, token_mask=parity(1))])
+    assert [[t % 2 for t in g] for g in got] == [[0] * 5, [1] * 5]

@@ -20,7 +20,7 @@ def mask_of(params: SamplingParams, made: Sequence[int], vocab: int) -> Optional
     mask = params.token_mask(list(made)) if params.token_mask is not None else None
     if mask is None:
         return None
-    mask, words = np.ascontiguousarray(mask), -(-vocab // 32)
+    mask, words = np.array(mask, order="C"), -(-vocab // 32)          # (a copy: a grammar may fill one array for several requests)
     if mask.dtype.itemsize != 4 or mask.dtype.kind not in "iu" or mask.shape != (words,):
         raise ValueError(f"a token mask is {words} 32-bit words for {vocab} tokens, got {mask.dtype} {mask.shape}")
     return mask
