@@ -100,3 +100,30 @@ def test_a_grammar_that_reuses_its_array(tmp_path, backend):
         return mask
     got = eng.generate([[1, 2, 3], [4, 5]], [SamplingParams(max_new_tokens=5, token_mask=parity(0)), SamplingParams(max_new_tokens=5, token_mask=parity(1))])
     assert [[t % 2 for t in g] for g in got] == [[0] * 5, [1] * 5]
+
+
+def test_a_mask_that_allows_nothing_is_none():
+    """Bits behind the vocabulary are no tokens.  (The draw from such a row would be token 0, which the grammar does not allow.)"""
+    from tffinfer_b200.sampling import mask_of
+    for vocab in (1, 31, 32, 33, 64, 70):
+        words = -(-vocab // 32)
+        none = np.zeros(words * 32, dtype=bool)
+        none[vocab:] = True
+        for empty in (np.zeros(words, np.int32), np.packbits(none, bitorder="little").view(np.uint32)):
+            with pytest.raises(ValueError, match="allows no token"):
+                mask_of(SamplingParams(token_mask=lambda made: empty), [], vocab)
+        for t in {0, vocab // 2, vocab - 1}:
+            some = np.zeros(words * 32, dtype=bool)
+            some[t] = True
+            got = mask_of(SamplingParams(token_mask=lambda made: np.packbits(some, bitorder="little").view(np.int32)), [], vocab)
+            assert got.view(np.uint32)[t // 32] == 1 << t % 32
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+def test_a_grammar_that_has_come_to_its_end(tmp_path, backend):
+    """It ends its request: nothing is drawn against it."""
+    eng = _engine(tmp_path, backend)
+    i = eng.add_request([1, 2, 3], SamplingParams(max_new_tokens=9, token_mask=lambda made: _even(made) if len(made) < 4 else np.zeros(WORDS, np.int32)))
+    while eng.has_unfinished():
+        eng.step()
+    assert eng.requests[i].finish_reason == "bad_mask" and [t % 2 for t in eng.requests[i].generated] == [0, 1, 0, 1]

@@ -23,6 +23,8 @@ def mask_of(params: SamplingParams, made: Sequence[int], vocab: int) -> Optional
     mask, words = np.array(mask, order="C"), -(-vocab // 32)          # (a copy: a grammar may fill one array for several requests)
     if mask.dtype.itemsize != 4 or mask.dtype.kind not in "iu" or mask.shape != (words,):
         raise ValueError(f"a token mask is {words} 32-bit words for {vocab} tokens, got {mask.dtype} {mask.shape}")
+    if not mask[:-1].any() and not int(mask.view(np.uint32)[-1]) << (32 * words - vocab) & 0xffffffff:
+        raise ValueError(f"a token mask allows no token of {vocab}")
     return mask
 
 

@@ -37,7 +37,7 @@ class SamplingParams:
     presence_penalty: float = 0.0      # taken off a token's logit once it was generated
     logit_bias: Tuple[Tuple[int, float], ...] = ()        # (token, what is added to its logit; -infinity bans it)
     # a grammar: the generated tokens so far -> 32-bit words with a bit for every allowed token (token t: bit t % 32 of word
-    # t // 32), or None for no limit.  At least one token is allowed.  Where it raises, or gives something else, its request ends (Engine:
+    # t // 32), or None for no limit.  Where it raises, allows no token or gives something else, its request ends (Engine:
     # reason "bad_mask")
     token_mask: Optional[Callable[[List[int]], Optional[np.ndarray]]] = None
 
