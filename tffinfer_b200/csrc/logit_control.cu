@@ -74,10 +74,10 @@ __device__ __noinline__ float divided(float x, float by) { return x / by; }
 
 // A request's penalties, with the operations of repetition_penalty_kernel (sampling.cu): a request's logits are the same, bit by bit,
 // whichever of the two kernels its step takes.  A quotient rounded once, at two products more than x * (1 / repetition) takes: with the
-// reciprocal y rounded to nearest, q = x y and the remainder r = x - q repetition (exact in an fma), q + r y is x / repetition
-// rounded to nearest where nothing over- or underflows (P. Markstein, Computation of elementary functions on the IBM RISC System/6000,
-// 1990).  64 rows 27.5 us, the nodes of eight trees 64.5; with a division for every such logit 28.1 and 72, with x y alone, a rounding more,
-// 24.9 and 56.
+// reciprocal y rounded to nearest, q = x y and the remainder r = x - q repetition, q + r y is x / repetition rounded to nearest (after
+// P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990; compared with the division for all 2^46 pairs of
+// significands) where nothing over- or underflows.  When it was brought in: 64 rows 27.5 us, the nodes of eight trees 64.5; with a
+// division for every such logit 28.1 and 72, with x y alone, a rounding more, 24.9 and 56.
 struct Penalties {
     float rep, inverse, freq, pres;
     unsigned quick;                                  // QUICK, or 0: this penalty is divided by
@@ -163,7 +163,8 @@ __global__ void __launch_bounds__(NT, CTAS_AN_SM) control_kernel(const ControlPa
         __syncthreads();                             // (the part before is through with the counts)
         // The first history tokens, the masks of the first rows and the counts' zeros are on their way together.
         const int* at = p.history + first_token;
-        const int skew = len > 0 ? (int)((uintptr_t)at >> 2 & 3) : 0, warp0 = tid & ~31;       // (without tokens nothing is loaded: the start may be any number)
+        // (without tokens nothing is loaded: their start may be any number)
+        const int skew = len > 0 ? (int)((uintptr_t)at >> 2 & 3) : 0, warp0 = tid & ~31;
         int4 t4[4];
         auto tokens_of = [&](int g0) {               // four tokens a load, from the 16 bytes on in which the history begins
 #pragma unroll

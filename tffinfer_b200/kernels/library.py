@@ -2105,8 +2105,8 @@ class CudaKernels:
         T, K = h.shape
         if isinstance(h, DeferredNorm):
             h = h.materialize()
-        # The fused form runs on pairs of SMs only, and writes keys and values where the positions say.  Where another configuration saves more waves than the separate
-        # kernel costs (a pass over the float32 projection at about 5 TB/s and a launch), the projection is not fused.
+        # The fused form runs on pairs of SMs only, and writes keys and values where the positions say.  Where another configuration saves more
+        # waves than the separate kernel costs (a pass over the float32 projection at about 5 TB/s and a launch), the projection is not fused.
         if self.USE_SM_PAIRS and T > self.SWAP_MAX_M and getattr(batch, "cache_slots", None) is None:
             costs = self.prompt_costs(T, (nq + 2 * nkv) * d, K, False)
             apart = min(v[0] for v in costs.values()) + T * (nq + 2 * nkv) * d * 6 / 5e6 + 3.0

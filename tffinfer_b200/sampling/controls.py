@@ -51,7 +51,8 @@ class LogitControls:
                                 not in [0, M); without mask_row it has mask r
     parents [R], tokens [R]     the rows of a request are the nodes of a tree of drafted tokens: parents as in
                                 ``CudaKernels.attention_tree``, and as many as there are (a tree of more than 256 takes longer a
-                                node).  A row's path is its node and that node's ancestors
+                                node).  A row's path is its node and that node's ancestors; node 0, the token drawn last, is on every
+                                path, and so not in the history
     """
     row_start: torch.Tensor
     settings: torch.Tensor
