@@ -285,3 +285,37 @@ def test_generation_over_trees_gives_the_tokens_of_single_steps(tmp_path):
             held[b] += e[:n]
     assert [m[:goal] for m in made] == single and steps < goal * 0.7
     run.ops.check_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 48])
+def test_arrays_of_a_larger_step_write_nothing_behind_this_one(ops, dtype, d):
+    """A captured step whose arrays are exchanged for those of more nodes than it has rows: the rows that it has are right, those behind stay."""
+    nq, nkv, T = 4, 2, 11
+    gen = torch.Generator().manual_seed(d)
+    rand = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(DEV)
+    cache, bt = rand(16, 1, 2, nkv, 16, d), i32(np.arange(16).reshape(4, 4))
+    trees = [[-1, 0, 0], [-1, 0, 1, 1, 0], [-1, 0, 0, 1, 1, 2], [-1, 0]]        # 16 nodes: three of the third request's rows are there
+    q, parents = rand(T, nq * d), i32(np.concatenate(trees)[:T])
+    ctx, n = [5, 30, 20, 9], [len(t) for t in trees]
+    for part in (dict(), dict(whole=0), dict(splits=2)):
+        tc, general = ops._attention_tree_tc, ops._attention_tree_plain
+        try:
+            if "whole" in part:
+                ops._attention_tree_tc = lambda *a: tc(*a, whole=0, least=1)
+            if "splits" in part:
+                ops._attention_tree_tc = lambda *a: False
+                ops._attention_tree_plain = lambda *a: general(*a, splits=2)
+            outs = []
+            for counts in (n, [3, 5, 3]):
+                batch = step_batch(ctx[:len(counts)], counts)
+                store = torch.full((T + 8, nq * d), 7.0, dtype=dtype, device=DEV)
+                ops.attention_tree(q, batch, parents, bt, cache, 0, 16, store[:T], nq, nkv, d, d, d ** -0.5)
+                torch.cuda.synchronize()
+                ops.check_errors()
+                assert (store[T:] == 7).all()
+                outs.append(store[:T].float())
+            assert (outs[0] - outs[1]).abs().max() <= (2.0 ** -17 if dtype == torch.float32 else 2.0 ** -6) * outs[1].abs().max()
+        finally:
+            for name in ("_attention_tree_tc", "_attention_tree_plain"):
+                ops.__dict__.pop(name, None)

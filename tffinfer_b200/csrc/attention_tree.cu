@@ -29,7 +29,7 @@ constexpr int BLOCK = 32, JOIN_THREADS = 128, NODE_WORDS = TREE_MAX_NODES / 32;
 
 struct TreeParams {
     const int *q_start, *pos_start, *parents, *block_table;
-    int table_width, pages, layer, nq, nkv, d, dv, window, keep, splits, stages, vec, q_vec;
+    int tokens, table_width, pages, layer, nq, nkv, d, dv, window, keep, splits, stages, vec, q_vec;
     float scale, softcap;
     int sink;
     const float *sink_val, *gate;
@@ -60,7 +60,7 @@ attention_tree_kernel(const T* q_in, const T* cache, T* __restrict__ out, const 
     float* sp = (float*)(sq + WARPS * RW * k4) + warp * RW * BLOCK;       // the warp's weights [RW][32]
     pdl_launch_dependents();
     pdl_wait();
-    const int q0 = p.q_start[b], nodes = min(p.q_start[b + 1] - q0, TREE_MAX_NODES), rows = nodes * G, row0 = blockIdx.x * WARPS * RW;
+    const int q0 = p.q_start[b], nodes = min(min(p.q_start[b + 1], p.tokens) - q0, TREE_MAX_NODES), rows = nodes * G, row0 = blockIdx.x * WARPS * RW;
     if (row0 >= rows) return;
     const int ctx = p.pos_start[b], hi = ctx + nodes - 1;
     const int lo_tile = p.window > 0 ? max(0, ctx - p.window + 1) : 0;    // the first position that a root sees
@@ -287,7 +287,7 @@ attention_tree_join_kernel(T* __restrict__ out, const TreeParams p) {
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.y, t = blockIdx.x / p.nq, h = blockIdx.x % p.nq, q0 = p.q_start[b], lane = threadIdx.x & 31;
-    if (t >= min(p.q_start[b + 1] - q0, TREE_MAX_NODES)) return;
+    if (t >= min(min(p.q_start[b + 1], p.tokens) - q0, TREE_MAX_NODES)) return;
     const size_t item = (size_t)(q0 + t) * p.nq + h;
     const float2 ml = lane < p.splits ? __ldcg((const float2*)p.part_ml + item * p.splits + lane) : make_float2(-INFINITY, 0.f);
     const float m = warp_max(ml.y > 0.f ? ml.x : -INFINITY);
@@ -383,7 +383,7 @@ TFF_API int tff_attention_tree(const void* q, int is_bf16, const int* q_start, c
     if (d > 512 || dv > 512 || max_nodes > TREE_MAX_NODES || (long long)requests * splits > 65535 || nkv > 65535)
         return TFF_ERR_UNSUPPORTED;
     TreeParams p = {};
-    p.q_start = q_start; p.pos_start = pos_start; p.parents = parents; p.block_table = block_table; p.table_width = table_width;
+    p.q_start = q_start; p.pos_start = pos_start; p.parents = parents; p.block_table = block_table; p.tokens = num_tokens; p.table_width = table_width;
     p.pages = (int)(cache_pages < 0x7fffffff ? cache_pages : 0x7fffffff);
     p.layer = layer; p.nq = nq; p.nkv = nkv; p.d = d; p.dv = dv;
     p.window = window > 0 ? window : 0; p.keep = window > 0 ? keep : 0;

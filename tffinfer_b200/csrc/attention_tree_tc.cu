@@ -26,7 +26,7 @@
 // 1,590, the products' and exponentials' time: a tree of 64 nodes behind 32,000 tokens (64/8 heads) 83 to 95 us by the clock
 // that the power cap leaves.  Around that, a CTA's first scores come 7,500 to 10,000 cycles after its start (2,900 for its place in the line, 3,500 for the
 // first keys), and a second piece costs about six blocks: 8 trees of 32 nodes behind 2,048 tokens 25.4 us, 71 MB.  Two tiles leave a thread 96
-// registers, and 92 bytes are spilled (heads of 128; 80 with heads of 64, none with one tile).
+// registers, and 68 bytes are spilled (heads of 128; 72 with heads of 64, none with one tile).
 //   - The queries go ahead of all but two blocks of keys: behind a full ring of every CTA's they came 7,000 cycles later.
 //   - A walk counts ``extra`` = 6 units more than its blocks: 3 gives 94.4 / 27.8 us (the long tree / the 8 trees), 5 and 7 92.3, 91.2 / 27.2, 27.3, and
 //     12 91.2 / 28.7.
@@ -63,7 +63,7 @@ constexpr float RESCALE_THRESHOLD = 8.0f;            // in log2 units
 struct TreeTcParams {
     bf16* out;
     const int *q_start, *pos_start, *parents, *block_table;
-    int requests, table_width, cache_layers, layer, page_shift, nq, nkv, window, keep, least, extra, whole;
+    int tokens, requests, table_width, cache_layers, layer, page_shift, nq, nkv, window, keep, least, extra, whole;
     int group; unsigned group_inverse;               // query heads a kv head, and what a row number is multiplied by for its node
     int tile_rows;                                   // of 128: whole nodes
     int pages, no_group;                             // of the cache; a group of rows behind its last, which reads as zeros
@@ -105,7 +105,7 @@ struct Walk {
     int q0 = 0, nodes = 0, ctx = 0, lo = 0, tiles = 0, count = 0;
     __device__ __forceinline__ void read(const TreeTcParams& p, int b, int tile_rows) {
         q0 = p.q_start[b];
-        nodes = max(0, min(p.q_start[b + 1] - q0, TREE_MAX_NODES));
+        nodes = max(0, min(min(p.q_start[b + 1], p.tokens) - q0, TREE_MAX_NODES));      // (no rows behind the step's)
         ctx = p.pos_start[b];
         lo = p.window > 0 ? max(0, ctx - p.window + 1) : 0;         // the first position that a root sees
         tiles = (nodes * p.group + tile_rows - 1) / tile_rows;
@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(JOIN_ROWS * 8) attn_tree_join_kernel(const Tre
     const int b = join.x, last = blockIdx.x;
     const int row = blockIdx.y * JOIN_ROWS + threadIdx.x % JOIN_ROWS, c = threadIdx.x / JOIN_ROWS * FOURS;
     const int R = (join.z * QT + row / BLOCK_M) * p.tile_rows + row % BLOCK_M;
-    const int q0 = p.q_start[b], rows_total = min(p.q_start[b + 1] - q0, TREE_MAX_NODES) * p.group;
+    const int q0 = p.q_start[b], rows_total = min(min(p.q_start[b + 1], p.tokens) - q0, TREE_MAX_NODES) * p.group;
     if (row % BLOCK_M >= p.tile_rows || R >= rows_total) return;
     float m = -INFINITY, l = 0.f;
     float4 o[FOURS];
@@ -800,7 +800,7 @@ TFF_API int tff_attention_tree_tc(const void* q, const int* q_start, const int* 
     TreeTcParams p = {};
     p.out = (bf16*)out;
     p.q_start = q_start; p.pos_start = pos_start; p.parents = parents; p.block_table = block_table;
-    p.requests = requests; p.table_width = table_width; p.cache_layers = cache_layers; p.layer = layer;
+    p.tokens = num_tokens; p.requests = requests; p.table_width = table_width; p.cache_layers = cache_layers; p.layer = layer;
     p.page_shift = page_size == 8 ? 3 : page_size == 16 ? 4 : page_size == 32 ? 5 : 6;
     p.nq = nq; p.nkv = nkv; p.window = window > 0 ? window : 0; p.keep = window > 0 ? keep : 0;
     p.least = least; p.extra = extra; p.whole = whole;
